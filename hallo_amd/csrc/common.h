@@ -116,8 +116,8 @@ __device__ __forceinline__ float gelu_u(float u) {
   return __builtin_fmaf(-au, __builtin_amdgcn_exp2f(q), fmaxf(u, 0.0f));
 }
 
-// Two gelu_u at once on the packed fp32 pipe (v_pk_fma_f32: two IEEE fmas per issue slot): the same operations in the same order
-// as gelu_u, element by element -- bit-identical results; |u|, max and the transcendental stay scalar.
+// Two gelu_u side by side: the same operations in the same order as gelu_u, element by element -- bit-identical results.  (Ordinary
+// scalar fmas: the build turns packed fp32 instructions off.)
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 __device__ __forceinline__ f32x2 pk_fma(f32x2 a, f32x2 b, f32x2 c) { return __builtin_elementwise_fma(a, b, c); }
 __device__ __forceinline__ f32x2 gelu_u2(f32x2 u) {

@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256) void ff320_kernel(const FfArgs p) {
   // GEGLU of one accumulator element pair: value register E, gate register E + 8 (common.h gelu_u: the scales ride in b1)
   f32x4 cb[2][4];                 // [chunk of the pair][value 0..3, value 8..11, gate 0..3, gate 8..11]
   float hf[16];
-  // elements E, E + 1 (E even) of chunk c at once: the fma / mul pairs issue on the packed fp32 pipe (common.h gelu_u2)
+  // elements E, E + 1 (E even) of chunk c at once: common.h gelu_u2
   auto geglu_pair = [&](auto e_c, const f32x16& acc, const int c) {
     constexpr int E = decltype(e_c)::value;
     static_assert((E & 1) == 0, "pair");
