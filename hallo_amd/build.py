@@ -12,8 +12,9 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhallo_amd.so")
-SOURCES = ["gemm.hip", "gemm3.hip", "gemm4.hip", "gemm_rs.hip", "gemm_rs2.hip", "gemm_ff.hip", "attention.hip", "attention40.hip", "fp8.hip", "fused_xattn.hip", "norm_elementwise.hip", "wav2vec.hip"]
-HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm_args.h"), os.path.join(CSRC, "attn_args.h"), os.path.join(HERE, "..", "include", "hallo_amd.h")]
+SOURCES = ["gemm.hip", "gemm3.hip", "gemm4.hip", "gemm_rs.hip", "gemm_rs2.hip", "gemm_ff.hip", "attention.hip", "attention40.hip", "fp8.hip", "fused_xattn.hip", "norm_elementwise.hip", "wav2vec.hip",
+           "norm_train.hip", "rope.hip", "window_attention.hip", "window_attention_bwd.hip"]
+HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm_args.h"), os.path.join(CSRC, "attn_args.h"), os.path.join(CSRC, "window_args.h"), os.path.join(HERE, "..", "include", "hallo_amd.h")]
 
 # No packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms give wrong results now and then on this hardware, and hipcc
 # -O3 forms them from ordinary float code.  The host pass warns that it does not know the feature; that is harmless.

@@ -1,0 +1,208 @@
+// Rotary positions over up to four axes (time, height, width, ...).
+//
+// Axis a owns d_a columns of every head, its pair i turns by pos_a * theta^(-2i / d_a):
+//   y_m = x_m cos - x_n sin,   y_n = x_n cos + x_m sin      (m, n) = (2i, 2i + 1) or (i, i + d_a / 2) within the axis' columns
+// Columns behind the last axis pass through.  The gradient of a rotation is the rotation by the negative angle (`inverse`).
+//
+// Angles: a frequency is a 64-bit fixed-point fraction of a turn, so pos * freq modulo 2^64 IS the angle modulo one turn -- exact for
+// every 32-bit position, where a 32-bit float product is off by whole radians near 10^7.  The top 32 bits go to sincospi.
+//
+// The kernel is bound by HBM (x read once, y written once).  A workgroup takes `tt` tokens: it computes their cos / sin once into LDS,
+// shared by all heads, then walks (token, head, unit); a unit is V columns and, in the half-split form, their V partners, so every
+// element is read and written by one thread (y may be x).  V = the largest of 8, 4, 2, 1 that divides the axes' (half) widths.
+#include "common.h"
+#include "../../include/hallo_amd.h"
+
+namespace hallo {
+
+namespace {
+
+constexpr int ROPE_MAX_HD = 256;
+constexpr int ROPE_PAIRS = 1024;                 // cos / sin pairs a workgroup holds (8 KB)
+constexpr int ROPE_TT = 64;                      // most tokens of a workgroup
+
+struct RopeArgs {
+  const void* x; void* y;
+  long x_bs, x_rs, y_bs, y_rs;
+  const unsigned long long* freq;                // [pairs] turns * 2^64
+  const int* pos; long pos_bs;                   // [B or 1, L, n_axes]; null: grid
+  int n_axes, dims[4], grid[4], origin[4];
+  int inverse, heads, hd, pairs, tt;
+  long L, tokens;                                // tokens = B * L
+};
+
+template <typename T, int V> struct __attribute__((aligned(2 * V))) PieceA { T v[V]; };
+template <typename T, int V> struct __attribute__((packed, aligned(2))) PieceU { T v[V]; };
+
+// IL: interleaved pairs.  AL: every piece of V columns is aligned to its size.
+template <typename T, int V, bool IL, bool AL>
+__global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
+  using P = typename std::conditional<AL, PieceA<T, V>, PieceU<T, V>>::type;
+  __shared__ float2 cs[ROPE_PAIRS];
+  __shared__ int ucol[ROPE_MAX_HD], upart[ROPE_MAX_HD], upair[ROPE_MAX_HD];    // unit: first column, partner column (-1: passes through), first pair
+  __shared__ long xoff[ROPE_TT], yoff[ROPE_TT];
+  const int tid = threadIdx.x;
+  const long t0 = (long)blockIdx.x * p.tt;
+  const int nt = (int)(p.tokens - t0 < p.tt ? p.tokens - t0 : p.tt);
+
+  // unit table (the axes' sections, then the columns that pass through)
+  int units = 0;
+  {
+    int col = 0, pair = 0;
+    for (int a = 0; a < p.n_axes; ++a) {
+      const int d = p.dims[a], n = (IL ? d : d / 2) / V;
+      for (int u = tid; u < n; u += 256) {
+        ucol[units + u] = col + u * V;
+        upart[units + u] = IL ? 0 : col + d / 2 + u * V;
+        upair[units + u] = pair + (IL ? u * V / 2 : u * V);
+      }
+      units += n; col += d; pair += d / 2;
+    }
+    const int n = (p.hd - col) / V;
+    for (int u = tid; u < n; u += 256) { ucol[units + u] = col + u * V; upart[units + u] = -1; upair[units + u] = 0; }
+    if (p.x != p.y) units += n;                  // in place they stay where they are
+  }
+  if (tid < nt) {
+    const long t = t0 + tid, b = t / p.L, l = t - b * p.L;
+    xoff[tid] = b * p.x_bs + l * p.x_rs;
+    yoff[tid] = b * p.y_bs + l * p.y_rs;
+  }
+  for (int k = tid; k < nt * p.pairs; k += 256) {
+    const int tt = k / p.pairs, j = k - tt * p.pairs;
+    const long t = t0 + tt, b = t / p.L, l = t - b * p.L;
+    int a = 0, first = 0;
+    while (j >= first + p.dims[a] / 2) { first += p.dims[a] / 2; ++a; }
+    int pos;
+    if (p.pos) pos = p.pos[b * p.pos_bs + l * p.n_axes + a];
+    else {
+      long r = l;
+      for (int c = p.n_axes - 1; c > a; --c) r /= p.grid[c];
+      pos = p.origin[a] + (int)(r % p.grid[a]);
+    }
+    const unsigned long long turn = (unsigned long long)(long long)pos * p.freq[j];
+    const float half_turns = (float)(int)(unsigned)(turn >> 32) * 0x1p-31f;
+    float s, c;
+    sincospif(half_turns, &s, &c);
+    cs[k] = make_float2(c, p.inverse ? -s : s);
+  }
+  __syncthreads();
+
+  const T* X = reinterpret_cast<const T*>(p.x);
+  T* Y = reinterpret_cast<T*>(p.y);
+  const unsigned per = (unsigned)(p.heads * units), items = per * (unsigned)nt;
+  constexpr int N = 4;                           // items a thread loads before it stores the first (x and y may be the same memory)
+  for (unsigned k0 = tid; k0 < items; k0 += 256 * N) {
+    P a[N], b[N];
+    unsigned tt[N], hh[N], un[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const unsigned k = k0 + 256 * i;
+      if (k >= items) break;
+      tt[i] = k / per;
+      const unsigned r = k - tt[i] * per;
+      hh[i] = r / (unsigned)units;
+      un[i] = r - hh[i] * (unsigned)units;
+      const T* xr = X + xoff[tt[i]] + (long)hh[i] * p.hd;
+      a[i] = *reinterpret_cast<const P*>(xr + ucol[un[i]]);
+      if (!IL && upart[un[i]] >= 0) b[i] = *reinterpret_cast<const P*>(xr + upart[un[i]]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (k0 + 256 * i >= items) break;
+      const int u = un[i], c0 = ucol[u], c1 = upart[u];
+      const float2* w = cs + tt[i] * p.pairs + upair[u];
+      T* yr = Y + yoff[tt[i]] + (long)hh[i] * p.hd;
+      if (c1 < 0) { *reinterpret_cast<P*>(yr + c0) = a[i]; continue; }
+      P o;
+      if constexpr (IL) {
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) {
+          const float2 t = w[e];
+          const float m = to_f32(a[i].v[2 * e]), n = to_f32(a[i].v[2 * e + 1]);
+          o.v[2 * e] = from_f32<T>(m * t.x - n * t.y);
+          o.v[2 * e + 1] = from_f32<T>(n * t.x + m * t.y);
+        }
+        *reinterpret_cast<P*>(yr + c0) = o;
+      } else {
+        P q;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float2 t = w[e];
+          const float m = to_f32(a[i].v[e]), n = to_f32(b[i].v[e]);
+          o.v[e] = from_f32<T>(m * t.x - n * t.y);
+          q.v[e] = from_f32<T>(n * t.x + m * t.y);
+        }
+        *reinterpret_cast<P*>(yr + c0) = o;
+        *reinterpret_cast<P*>(yr + c1) = q;
+      }
+    }
+  }
+}
+
+template <typename T, int V, bool IL>
+int launch_rope(const RopeArgs& a, bool al, hipStream_t st) {
+  const long grid = (a.tokens + a.tt - 1) / a.tt;
+  if (grid > 0x7fffffff) return -22;
+  if (al) hipLaunchKernelGGL((rope_kernel<T, V, IL, true>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((rope_kernel<T, V, IL, false>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  HALLO_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+int pick_rope(const RopeArgs& a, int V, bool il, bool al, hipStream_t st) {
+  if (il) return V == 8 ? launch_rope<T, 8, true>(a, al, st) : V == 4 ? launch_rope<T, 4, true>(a, al, st) : launch_rope<T, 2, true>(a, al, st);
+  return V == 8 ? launch_rope<T, 8, false>(a, al, st)
+                : V == 4 ? launch_rope<T, 4, false>(a, al, st) : V == 2 ? launch_rope<T, 2, false>(a, al, st) : launch_rope<T, 1, false>(a, al, st);
+}
+
+}  // namespace
+}  // namespace hallo
+
+extern "C" int hallo_rope(const hallo_rope_desc* d, void* stream) {
+  using namespace hallo;
+  if (!d || (d->dtype != DT_F16 && d->dtype != DT_BF16) || d->batch < 0 || d->L < 0 || d->heads < 1 || d->heads > (1 << 20) || d->head_dim < 2 || d->head_dim % 2 ||
+      d->head_dim > ROPE_MAX_HD || d->n_axes < 1 || d->n_axes > 4 || d->batch > 0x7fffffff)
+    return -22;
+  RopeArgs a = {};
+  int sum = 0, g = d->head_dim;                  // g: greatest common divisor that V has to divide
+  auto gcd = [](int x, int y) { while (y) { const int t = x % y; x = y; y = t; } return x; };
+  const bool il = d->interleaved != 0;
+  const bool none = d->batch == 0 || d->L == 0;
+  long cells = 1;
+  for (int i = 0; i < d->n_axes; ++i) {
+    if (d->dims[i] < 2 || d->dims[i] % 2 || d->dims[i] > ROPE_MAX_HD) return -22;
+    sum += d->dims[i];
+    g = gcd(g, il ? d->dims[i] : d->dims[i] / 2);
+    a.dims[i] = d->dims[i];
+    if (!d->pos && !none) {
+      if (d->grid[i] < 1 || cells > d->L / d->grid[i] + 1) return -22;
+      cells *= d->grid[i];
+      a.grid[i] = d->grid[i];
+      a.origin[i] = d->origin[i];
+    }
+  }
+  if (sum > d->head_dim || (!d->pos && !none && cells != d->L)) return -22;
+  const long width = (long)d->heads * d->head_dim;
+  if (d->x_rs < 0 || d->y_rs < width || d->L > (1L << 40) || (d->batch > 0 && d->L > (1L << 46) / d->batch)) return -22;
+  if (none) return 0;
+  if (!d->x || !d->y || !d->freq) return -22;
+  if (d->x == d->y && (d->x_bs != d->y_bs || d->x_rs != d->y_rs)) return -22;
+  a.x = d->x; a.y = d->y;
+  a.x_bs = d->x_bs; a.x_rs = d->x_rs; a.y_bs = d->y_bs; a.y_rs = d->y_rs;
+  a.freq = reinterpret_cast<const unsigned long long*>(d->freq);
+  a.pos = d->pos; a.pos_bs = d->pos_bs;
+  a.n_axes = d->n_axes; a.inverse = d->inverse != 0; a.heads = d->heads; a.hd = d->head_dim; a.pairs = sum / 2;
+  a.L = d->L; a.tokens = d->batch * d->L;
+  const int V = g % 8 == 0 ? 8 : g % 4 == 0 ? 4 : g % 2 == 0 ? 2 : 1;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) |
+                         (uintptr_t)(2 * (a.x_rs | a.y_rs | a.hd | (d->batch > 1 ? a.x_bs | a.y_bs : 0)));
+  const bool al = bits % (2 * V) == 0;
+  // tokens of a workgroup: enough to fill its lanes and the cos / sin table, few enough to spread over the 256 CUs
+  int tt = ROPE_PAIRS / a.pairs;
+  if (tt > ROPE_TT) tt = ROPE_TT;
+  while (tt > 1 && (a.tokens + tt - 1) / tt < 1024) tt = (tt + 1) / 2;
+  a.tt = tt;
+  hipStream_t st = (hipStream_t)stream;
+  return d->dtype == DT_F16 ? pick_rope<_Float16>(a, V, il, al, st) : pick_rope<__bf16>(a, V, il, al, st);
+}

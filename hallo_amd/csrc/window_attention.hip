@@ -1,0 +1,499 @@
+// Attention with a sliding window and always-visible first keys, shared key heads and per-entry lengths: forward pass.
+//
+// Two forms.  `win_fwd_kernel` takes 128 queries of one head per workgroup (a wave owns 32) and walks the keys those queries see; K and
+// V tiles go global -> registers -> LDS one tile ahead of the MFMAs.  `win_split_kernel` is for few queries (single tokens against a
+// cache): the query rows of the heads that share a key head are packed into one 32-row block, the keys are split over workgroups and
+// over the waves of each, and `win_join_kernel` joins the parts.
+//
+// Both contractions run in swapped form, so a lane owns a query and the softmax statistics are lane-local:
+//   S^T[key, q] = K[key, :] . Q[q, :]      A = K rows from LDS, B = Q fragments in registers
+//   O^T[d, q]   = V^T[d, :] . P^T[:, q]    A = V read transposed from LDS, B = P as the first product left it
+// The running maximum moves only when a score exceeds it by more than 6 (log2 units, so P <= 64 and the row sum stays far inside
+// fp32); P is rounded to the storage type for the second product only -- the row sum adds the unrounded values.
+#include <type_traits>
+#include "window_args.h"
+#include "../../include/hallo_amd.h"
+
+namespace hallo {
+
+namespace {
+
+template <typename T, int HK>
+__global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const WinArgs p) {
+  using V8 = typename Vec<T>::v8;
+  using V4 = typename Vec<T>::v4;
+  constexpr int KB = HK > 128 ? 32 : 64;         // keys per tile
+  constexpr int NT = KB / 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8;
+  constexpr int KP = win_pitch_row(HK), VP = win_pitch_tr(HK), STAGE = KB * (KP + VP);
+  constexpr int U = (KB * CH + 255) / 256;       // 16-byte pieces per thread and tensor
+  constexpr float NEG_INF = -__builtin_inff();
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+  win_lds* const lds = (win_lds*)smem;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hi = lane >> 5, l31 = lane & 31;
+  int bid = xcd_remap(blockIdx.x, p.batch * p.heads * p.nqb);      // the blocks of a key head stay in one XCD's L2
+  const int qb = p.nqb - 1 - bid % p.nqb;        // causal masks: the blocks with the most keys first
+  bid /= p.nqb;
+  const int h = bid % p.heads, b = bid / p.heads, hk = h / p.group;
+  const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk);
+  const T* Q = reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs;
+  const T* K = reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hk * p.k_hs;
+  const T* V = reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hk * p.v_hs;
+  const int i0 = qb * 128, iw = i0 + wave * 32, row = iw + l31;
+  const int shift = kn - qn;                     // position of query 0
+
+  V8 qf[NKS];
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    const int d = ks * 16 + hi * 8;
+    qf[ks] = row < qn && d < p.hd ? ld8<T>(Q + (long)row * p.q_rs + d) : zero8<T>();
+  }
+
+  WinRange r = {0, 0, 0};
+  if (i0 < qn) r = win_range(p, shift + i0, shift + min(i0 + 127, qn - 1), kn);
+  const int n0 = (r.e0 + KB - 1) / KB, nt = n0 + (r.e1 - r.s1 + KB - 1) / KB;
+  // this wave's positions and this lane's visible keys
+  const int pw0 = shift + iw, pw1 = shift + min(iw + 31, qn - 1), pos = shift + row;
+  const int vhi = p.right < 0 ? kn : min(kn, pos + p.right + 1), vlo = p.left < 0 ? 0 : pos - p.left;
+
+  V8 kr[U], vr[U];
+  unsigned ko[U], vo[U];                         // element offsets inside a tile (row strides are at most WIN_MAX_STRIDE)
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+    ko[i] = (unsigned)rr * (unsigned)p.k_rs + ch * 8;
+    vo[i] = (unsigned)rr * (unsigned)p.v_rs + ch * 8;
+  }
+  auto load = [&](int t) {
+    const int j0 = t < n0 ? t * KB : r.s1 + (t - n0) * KB, rem = (t < n0 ? r.e0 : r.e1) - j0;
+    const T* kt = K + (long)j0 * p.k_rs;
+    const T* vt = V + (long)j0 * p.v_rs;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+      const bool ok = rr < rem && rr < KB && ch * 8 < p.hd;        // rows past the range hold anything: they enter the products as zeros
+      kr[i] = ok ? ld8<T>(kt + ko[i]) : zero8<T>();
+      vr[i] = ok ? ld8<T>(vt + vo[i]) : zero8<T>();
+    }
+  };
+  auto store = [&](int stage) {
+    win_lds* const kt = lds + stage * STAGE;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+      if (KB * CH % 256 == 0 || u < KB * CH) {
+        *(__attribute__((address_space(3))) V8*)(kt + rr * KP + ch * 16) = kr[i];
+        *(__attribute__((address_space(3))) V8*)(kt + KB * KP + rr * VP + ch * 16) = vr[i];
+      }
+    }
+  };
+
+  f32x16 o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
+  float m = NEG_INF, l = 0.0f;
+  const float c = p.c, slack = 6.0f / p.c;
+  const f32x16 zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  const int kfo = l31 * KP + hi * 16;
+  const int vfo = (4 * hi + ((lane & 15) >> 2)) * VP + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+
+  if (nt > 0) { load(0); store(0); }
+  if (nt > 1) load(1);
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    const int j0 = t < n0 ? t * KB : r.s1 + (t - n0) * KB, end = t < n0 ? r.e0 : r.e1;
+    if (t + 1 < nt) store((t + 1) & 1);          // read last in iteration t - 1, which the barrier below closed
+    if (t + 2 < nt) load(t + 2);
+    const win_lds* const kt = lds + (t & 1) * STAGE;
+    const win_lds* const vt = kt + KB * KP;
+    const bool none = iw >= qn || (p.right >= 0 && j0 > pw1 + p.right) || (p.left >= 0 && j0 + KB <= pw0 - p.left && j0 >= p.sinks);
+    if (!none) {
+      f32x16 s[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[n] = zero16;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks)
+          s[n] = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(kt + kfo + n * 32 * KP + ks * 32), qf[ks], s[n]);
+      }
+      const bool all = end - j0 >= KB && (p.right < 0 || j0 + KB - 1 <= pw0 + p.right) &&
+                       (p.left < 0 || j0 >= pw1 - p.left || j0 + KB <= p.sinks);
+      if (!all) {
+        const int lhi = min(vhi, end);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int j = j0 + n * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi;
+            s[n][e] = j < lhi && (j >= vlo || j < p.sinks) ? s[n][e] : NEG_INF;
+          }
+      }
+      float mt = NEG_INF;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[n][e]);
+      mt = win_half_max(mt);
+      if (__any(mt > m + slack)) {
+        const float mn = fmaxf(m, mt);
+        const float a = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);     // m = -inf: 0
+        m = mn;
+        l *= a;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[db][e] *= a;
+      }
+      const float mc = m == NEG_INF ? 0.0f : m * c;
+      V8 pf[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], c, -mc));
+          l += pv;
+          pf[n][e >> 3][e & 7] = from_f32<T>(pv);
+        }
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const int colb = min(db * 32 + gdh * 16, HK - 16) * 2;     // columns past HK: rows of O^T that are not stored
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2)
+            o[db] = Vec<T>::mfma32(win_tr8<V8, VP>(vt + vfo, n * 32 + h2 * 16, colb), pf[n][h2], o[db]);
+      }
+    }
+    __syncthreads();
+  }
+
+  l = win_half_sum(l);
+  if (row >= p.Lq) return;
+  const bool some = row < qn && l > 0.0f;
+  // a NaN sum stays NaN
+  const float inv = some ? 1.0f / l : (l != l && row < qn ? l : 0.0f);
+  if (p.lse && hi == 0)
+    p.lse[((long)b * p.heads + h) * p.Lq + row] = some ? (m * c + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f : (inv != 0.0f ? inv : NEG_INF);
+  T* O = reinterpret_cast<T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)row * p.o_rs;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = db * 32 + 8 * g + 4 * hi;
+      if (d < p.hd) {
+        V4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(inv == 0.0f ? 0.0f : o[db][4 * g + e] * inv);
+        *reinterpret_cast<V4*>(O + d) = w;
+      }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------
+// Few queries.  Row r of a block of 32 is query r % Lq of head hk * group + r / Lq.  Bound by the bytes of K and V: a wave reads 32 keys
+// at a time, K straight into MFMA operands (lane = key row), V through an LDS tile of its own (no barrier), the next 32 keys in
+// flight under the products; the four waves take every fourth tile of the split and join through LDS.
+// ------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int HK>
+__global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
+  using V8 = typename Vec<T>::v8;
+  constexpr int NKS = HK / 16, NDB = (HK + 31) / 32, VP = win_pitch_tr(HK), OP = HK + 4;      // OP: pitch of the joined rows, floats
+  constexpr float NEG_INF = -__builtin_inff();
+  constexpr int VT = 4 * 32 * VP, JT = 32 * OP * 4;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[VT > JT ? VT : JT];
+  __shared__ float sm_m[4][32], sm_l[4][32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hi = lane >> 5, l31 = lane & 31;
+  int bid = blockIdx.x;
+  const int split = bid % p.nsplit; bid /= p.nsplit;
+  const int rb = bid % p.nrb; bid /= p.nrb;
+  const int hk = bid % p.kv_heads, b = bid / p.kv_heads;
+  const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk), shift = kn - qn;
+  const int rows = p.group * p.Lq, r = rb * 32 + l31, gh = r / p.Lq, i = r - gh * p.Lq;
+  const bool live = r < rows && i < qn;
+  const T* K = reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hk * p.k_hs;
+  const T* V = reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hk * p.v_hs;
+  const T* Qr = reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)(hk * p.group + gh) * p.q_hs + (long)i * p.q_rs;
+  V8 qf[NKS];
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    const int d = ks * 16 + hi * 8;
+    qf[ks] = live && d < p.hd ? ld8<T>(Qr + d) : zero8<T>();
+  }
+  // the queries of this block: all of them once it reaches over a head's end
+  const int last = min(rb * 32 + 31, rows - 1), ilo = rb * 32 / p.Lq == last / p.Lq ? rb * 32 % p.Lq : 0,
+            ihi = min(rb * 32 / p.Lq == last / p.Lq ? last % p.Lq : p.Lq - 1, qn - 1);
+  WinRange w = {0, 0, 0};
+  if (ihi >= ilo) w = win_range(p, shift + ilo, shift + ihi, kn);
+  const int n0 = (w.e0 + 31) / 32, nt = n0 + (w.e1 - w.s1 + 31) / 32;
+  const int tb = (int)((long)nt * split / p.nsplit), te = (int)((long)nt * (split + 1) / p.nsplit);
+  const int pos = shift + i;
+  const int vhi = !live ? 0 : (p.right < 0 ? kn : min(kn, pos + p.right + 1)), vlo = p.left < 0 ? 0 : pos - p.left;
+  const int plo = shift + ilo, phi = shift + ihi;
+
+  V8 kr[NKS], vr[NKS];
+  auto load = [&](int t) {
+    const int j0 = t < n0 ? t * 32 : w.s1 + (t - n0) * 32, rem = (t < n0 ? w.e0 : w.e1) - j0;
+    const T* kt = K + (long)(j0 + l31) * p.k_rs + hi * 8;
+    const T* vt = V + (long)(j0 + l31) * p.v_rs + hi * 8;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const bool ok = l31 < rem && ks * 16 + hi * 8 < p.hd;
+      kr[ks] = ok ? ld8<T>(kt + ks * 16) : zero8<T>();
+      vr[ks] = ok ? ld8<T>(vt + ks * 16) : zero8<T>();
+    }
+  };
+  f32x16 o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
+  float m = NEG_INF, l = 0.0f;
+  const float c = p.c;
+  win_lds* const vt = (win_lds*)smem + wave * 32 * VP;
+  const int vfo = (4 * hi + ((lane & 15) >> 2)) * VP + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+
+  int t = tb + wave;
+  if (t < te) load(t);
+  for (; t < te; t += 4) {
+    f32x16 s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(kr[ks], qf[ks], s);
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) *(__attribute__((address_space(3))) V8*)(vt + l31 * VP + (ks * 16 + hi * 8) * 2) = vr[ks];
+    const int j0 = t < n0 ? t * 32 : w.s1 + (t - n0) * 32, end = t < n0 ? w.e0 : w.e1;
+    if (t + 4 < te) load(t + 4);
+    const bool all = end - j0 >= 32 && (p.right < 0 || j0 + 31 <= plo + p.right) && (p.left < 0 || j0 >= phi - p.left || j0 + 32 <= p.sinks);
+    if (!all) {
+      const int lhi = min(vhi, end);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = j0 + (e & 3) + 8 * (e >> 2) + 4 * hi;
+        s[e] = j < lhi && (j >= vlo || j < p.sinks) ? s[e] : NEG_INF;
+      }
+    }
+    float mt = NEG_INF;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[e]);
+    mt = win_half_max(mt);
+    if (__any(mt > m)) {
+      const float mn = fmaxf(m, mt);
+      const float a = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[db][e] *= a;
+    }
+    const float mc = m == NEG_INF ? 0.0f : m * c;
+    V8 pf[2];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -mc));
+      l += pv;
+      pf[e >> 3][e & 7] = from_f32<T>(pv);
+    }
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const int colb = min(db * 32 + gdh * 16, HK - 16) * 2;
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) o[db] = Vec<T>::mfma32(win_tr8<V8, VP>(vt + vfo, h2 * 16, colb), pf[h2], o[db]);
+    }
+  }
+  l = win_half_sum(l);
+  if (!live) { m = NEG_INF; l = 0.0f; }          // rows without a query went along in the tiles that need no mask
+  if (hi == 0) { sm_m[wave][l31] = m; sm_l[wave][l31] = l; }
+  __syncthreads();                               // also: every wave is done with its V tile, the joined rows take its place
+  const float M = fmaxf(fmaxf(sm_m[0][l31], sm_m[1][l31]), fmaxf(sm_m[2][l31], sm_m[3][l31]));
+  const float f = m == M ? 1.0f : __builtin_amdgcn_exp2f((m - M) * c);        // this wave's share (a wave without a visible key: o = 0)
+  float* const jt = reinterpret_cast<float*>(smem);
+  for (int w4 = 0; w4 < 4; ++w4) {
+    if (wave == w4) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d = db * 32 + 8 * g + 4 * hi;
+          if (d < HK) {
+            f32x4* a = reinterpret_cast<f32x4*>(jt + l31 * OP + d);
+            f32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = live ? o[db][4 * g + e] * f : 0.0f;
+            if (w4) x += *a;
+            *a = x;
+          }
+        }
+    }
+    __syncthreads();
+  }
+  // thread -> (row, 32 threads' stride over the columns)
+  const int rr = tid >> 3, cc = tid & 7, R = rb * 32 + rr;
+  float Mr = NEG_INF, Lr = 0.0f;
+#pragma unroll
+  for (int w4 = 0; w4 < 4; ++w4) Mr = fmaxf(Mr, sm_m[w4][rr]);
+#pragma unroll
+  for (int w4 = 0; w4 < 4; ++w4) Lr += sm_l[w4][rr] * (sm_m[w4][rr] == Mr ? 1.0f : __builtin_amdgcn_exp2f((sm_m[w4][rr] - Mr) * c));
+  if (R >= rows) return;
+  if (p.nsplit > 1) {
+    float* part = p.part + (((long)(b * p.kv_heads + hk) * p.nrb + rb) * p.nsplit + split) * 32 * (p.hd + 2) + rr * (p.hd + 2);
+    for (int d = cc; d < p.hd; d += 8) part[2 + d] = jt[rr * OP + d];
+    if (cc == 0) { part[0] = Mr; part[1] = Lr; }
+    return;
+  }
+  const int gr = R / p.Lq, ir = R - gr * p.Lq, h = hk * p.group + gr;
+  const float inv = Lr > 0.0f ? 1.0f / Lr : (Lr != Lr ? Lr : 0.0f);
+  T* O = reinterpret_cast<T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)ir * p.o_rs;
+  for (int d = cc * 8; d < p.hd; d += 64) {
+    V8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = from_f32<T>(inv == 0.0f ? 0.0f : jt[rr * OP + d + e] * inv);
+    st8<T>(O + d, x);
+  }
+  if (p.lse && cc == 0)
+    p.lse[((long)b * p.heads + h) * p.Lq + ir] = Lr > 0.0f ? (Mr * c + __builtin_amdgcn_logf(Lr)) * 0.69314718055994530942f : (inv != 0.0f ? inv : NEG_INF);
+}
+
+// one wave per query row: joins the parts of its key splits
+template <typename T>
+__global__ __launch_bounds__(256) void win_join_kernel(const WinArgs p) {
+  const int lane = threadIdx.x & 63;
+  const int rows = p.group * p.Lq;
+  const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (long)p.batch * p.kv_heads * rows) return;
+  const int R = (int)(id % rows);
+  const long bh = id / rows;
+  const int hk = (int)(bh % p.kv_heads), b = (int)(bh / p.kv_heads);
+  const int step = 32 * (p.hd + 2);
+  const float* part = p.part + (bh * p.nrb + R / 32) * p.nsplit * step + (R % 32) * (p.hd + 2);
+  float M = -__builtin_inff();
+  for (int s = lane; s < p.nsplit; s += 64) M = fmaxf(M, part[(long)s * step]);
+  M = wave_max(M);
+  float L = 0.0f, acc[3] = {0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float* q = part + (long)s * step;
+    const float f = q[0] == M ? 1.0f : __builtin_amdgcn_exp2f((q[0] - M) * p.c);
+    L += q[1] * f;
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (lane + 64 * k < p.hd) acc[k] += q[2 + lane + 64 * k] * f;
+  }
+  const int gr = R / p.Lq, i = R - gr * p.Lq, h = hk * p.group + gr;
+  const float inv = L > 0.0f ? 1.0f / L : (L != L ? L : 0.0f);
+  T* O = reinterpret_cast<T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)i * p.o_rs;
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    if (lane + 64 * k < p.hd) O[lane + 64 * k] = from_f32<T>(inv == 0.0f ? 0.0f : acc[k] * inv);
+  if (p.lse && lane == 0)
+    p.lse[((long)b * p.heads + h) * p.Lq + i] = L > 0.0f ? (M * p.c + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f : (inv != 0.0f ? inv : -__builtin_inff());
+}
+
+// Which form, and how many key splits.
+void plan(WinArgs& a) {
+  a.nqb = (a.Lq + 127) / 128;
+  a.nrb = (a.group * a.Lq + 31) / 32;
+  a.nsplit = 0;                                  // 0: 128-query blocks
+  const long blocks = (long)a.batch * a.heads * a.nqb;
+  if (a.Lq > 32 && blocks >= 128) return;
+  long keys = a.Lk;
+  if (a.left >= 0 && a.right >= 0) keys = (long)a.left + a.right + a.Lq + a.sinks;
+  if (keys > a.Lk) keys = a.Lk;
+  const long wgs = (long)a.batch * a.kv_heads * a.nrb, tiles = (keys + 31) / 32;
+  long ns = (512 + wgs - 1) / wgs;
+  if (ns > tiles / 8) ns = tiles / 8;
+  a.nsplit = ns < 1 ? 1 : (int)ns;
+}
+
+template <typename T, int HK>
+int launch_hk(const WinArgs& a, hipStream_t st) {
+  if (a.nsplit == 0) {
+    hipLaunchKernelGGL((win_fwd_kernel<T, HK>), dim3((unsigned)(a.batch * a.heads * a.nqb)), dim3(256), 0, st, a);
+    HALLO_CHECK_LAUNCH();
+    return 0;
+  }
+  hipLaunchKernelGGL((win_split_kernel<T, HK>), dim3((unsigned)(a.batch * a.kv_heads * a.nrb * a.nsplit)), dim3(256), 0, st, a);
+  HALLO_CHECK_LAUNCH();
+  if (a.nsplit > 1) {
+    const long rows = (long)a.batch * a.heads * a.Lq;
+    hipLaunchKernelGGL((win_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+    HALLO_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+template <typename T>
+int launch(const WinArgs& a, hipStream_t st) {
+  switch ((a.hd + 15) / 16) {
+    case 1: return launch_hk<T, 16>(a, st);
+    case 2: return launch_hk<T, 32>(a, st);
+    case 3: return launch_hk<T, 48>(a, st);
+    case 4: return launch_hk<T, 64>(a, st);
+    case 5: return launch_hk<T, 80>(a, st);
+    case 6: return launch_hk<T, 96>(a, st);
+    case 7: return launch_hk<T, 112>(a, st);
+    case 8: return launch_hk<T, 128>(a, st);
+    case 9: return launch_hk<T, 144>(a, st);
+    default: return launch_hk<T, 160>(a, st);
+  }
+}
+
+}  // namespace
+
+// shared with the backward pass: checks the sizes, strides and alignment of a descriptor and fills the arguments; false = refused
+bool win_args(const hallo_window_attn_desc* d, WinArgs& a) {
+  if (!d || (d->dtype != DT_F16 && d->dtype != DT_BF16) || d->batch < 0 || d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads ||
+      d->head_dim < 8 || d->head_dim > WIN_MAX_HD || d->head_dim % 8 || d->Lq < 0 || d->Lk < 0 || d->Lq > WIN_MAX_LEN || d->Lk > WIN_MAX_LEN ||
+      d->sinks < 0 || !(d->scale > 0.0f) || !(d->scale < 1e30f))
+    return false;
+  const int64_t strides[] = {d->q_bs, d->q_rs, d->q_hs, d->k_bs, d->k_rs, d->k_hs, d->v_bs, d->v_rs, d->v_hs, d->o_bs, d->o_rs, d->o_hs};
+  for (int64_t s : strides)
+    if (s < 0 || s % 8) return false;
+  const int64_t row_strides[] = {d->q_rs, d->k_rs, d->v_rs, d->o_rs};
+  for (int64_t s : row_strides)
+    if (s > WIN_MAX_STRIDE) return false;
+  const void* ptrs[] = {d->q, d->k, d->v, d->o};
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) & 15) return false;
+  if ((int64_t)d->batch * d->heads * ((d->Lq + 31) / 32) > 0x7fffffff || (int64_t)d->heads * d->Lq > 0x7fffffff ||
+      (int64_t)d->batch * d->heads * ((d->Lk + 31) / 32) > 0x7fffffff)
+    return false;
+  const auto cut = [](int x) { return x > WIN_MAX_LEN ? WIN_MAX_LEN : x; };
+  a = WinArgs{};
+  a.q = d->q; a.k = d->k; a.v = d->v; a.o = d->o; a.lse = d->lse;
+  a.q_bs = d->q_bs; a.q_rs = d->q_rs; a.q_hs = d->q_hs; a.k_bs = d->k_bs; a.k_rs = d->k_rs; a.k_hs = d->k_hs;
+  a.v_bs = d->v_bs; a.v_rs = d->v_rs; a.v_hs = d->v_hs; a.o_bs = d->o_bs; a.o_rs = d->o_rs; a.o_hs = d->o_hs;
+  a.q_len = d->q_len; a.kv_len = d->kv_len;
+  a.batch = d->batch; a.heads = d->heads; a.kv_heads = d->kv_heads; a.group = d->heads / d->kv_heads; a.hd = d->head_dim;
+  a.Lq = (int)d->Lq; a.Lk = (int)d->Lk;
+  a.left = d->left < 0 ? -1 : cut(d->left); a.right = d->right < 0 ? -1 : cut(d->right); a.sinks = cut(d->sinks);
+  a.scale = d->scale; a.c = d->scale * 1.44269504088896340736f;
+  return true;
+}
+
+}  // namespace hallo
+
+extern "C" int64_t hallo_window_attention_workspace(const hallo_window_attn_desc* d) {
+  using namespace hallo;
+  WinArgs a;
+  if (!win_args(d, a)) return -22;
+  if (a.batch == 0 || a.Lq == 0) return 0;
+  plan(a);
+  return a.nsplit > 1 ? (int64_t)a.batch * a.kv_heads * a.nrb * a.nsplit * 32 * (a.hd + 2) * 4 : 0;
+}
+
+extern "C" int hallo_window_attention(const hallo_window_attn_desc* d, void* stream) {
+  using namespace hallo;
+  WinArgs a;
+  if (!win_args(d, a)) return -22;
+  if (a.batch == 0 || a.Lq == 0) return 0;
+  if (!a.q || !a.o || (a.Lk > 0 && (!a.k || !a.v))) return -22;
+  const int64_t need = hallo_window_attention_workspace(d);
+  if (need > 0 && (!d->workspace || d->workspace_bytes < need)) return -22;
+  plan(a);
+  a.part = (float*)d->workspace;
+  if ((int64_t)a.batch * a.kv_heads * a.nrb * (a.nsplit > 0 ? a.nsplit : 1) > 0x7fffffff) return -22;
+  return d->dtype == DT_F16 ? launch<_Float16>(a, (hipStream_t)stream) : launch<__bf16>(a, (hipStream_t)stream);
+}

@@ -1,0 +1,581 @@
+// Attention with a sliding window and always-visible first keys: backward pass.
+//
+//   P = exp(scale q k^T - lse) over the visible pairs,   delta = sum_d(do * o)
+//   dV = P^T dO,   dS = P * (dO V^T - delta),   dQ = scale dS K,   dK = scale dS^T Q
+// summed over the query heads that share a key head.  Three launches, four with split keys:
+//   prep   delta and lse * log2(e) of every query (fp32; +inf where a query has no visible key, so its P is 0)
+//   dkv    a workgroup owns 128 keys (a wave 32): K and V stay in registers as MFMA operands, dK and dV as accumulators, and the query
+//          rows that see the keys stream through LDS, for all heads of the group -- shared heads need no atomics
+//   dq     a workgroup owns 128 queries of a head (a wave 32), the visible keys stream through LDS
+//   join   the sinks are seen by every query: their key tiles' query rows are split over workgroups, fp32 parts are added here in order
+//          (also used for all keys when there are too few key tiles to fill the chip)
+// S and dO V^T are computed in both dkv and dq (7 products where 5 would do with atomics on dQ): results do not depend on timing.
+//
+// fp16: P is 1/N over long rows and dS smaller still, below fp16's normal numbers.  Both are carried scaled by powers of two that cannot
+// overflow and are taken out of the fp32 accumulators at the end: P by 2^14 (P <= 1), dS by 2^e with |dS| <= 2 |do_i|_2 |v_j|_2 <
+// 2^(15 - e) -- in dkv the norm of the lane's own key row and the largest |do_i|, in dq the norm of the lane's own do row and the
+// largest |v_j|.  bf16 has fp32's range and needs neither.
+#include <type_traits>
+#include "window_args.h"
+#include "../../include/hallo_amd.h"
+
+namespace hallo {
+
+bool win_args(const hallo_window_attn_desc* d, WinArgs& a);      // window_attention.hip
+
+namespace {
+
+struct WinBwdArgs {
+  WinArgs w;
+  const void* dout; void *dq, *dk, *dv;
+  long do_bs, do_rs, do_hs, dq_bs, dq_rs, dq_hs, dk_bs, dk_rs, dk_hs, dv_bs, dv_rs, dv_hs;
+  float *delta, *lse2;                           // [batch, heads, Lq]
+  float *domax, *vmax;                           // fp16: largest row norms of 64 rows, [batch, heads, nq64], [batch, kv_heads, nk64]
+  int nq64, nk64;
+  int nst, nrt, sps, spr;                        // key tiles of the sinks / of the rest, query splits of each
+  float* part;                                   // [batch, kv_heads][nst * sps (if sps > 1) + nrt * spr (if spr > 1)][128][2 hd]
+  int nparts;                                    // part tiles of one (batch entry, key head)
+};
+
+constexpr int BW_KEYS = 128;                     // keys of a dkv workgroup
+constexpr float P_EXP = 14.0f;                   // fp16: P is carried times 2^14
+
+// 2^e with 2 a b 2^e < 2^15
+__device__ __forceinline__ float ds_scale(float a, float b) {
+  const float bound = 2.0f * a * b;
+  if (!(bound > 0.0f) || !(bound < 1e30f)) return 1.0f;
+  const int e = 15 - __builtin_amdgcn_frexp_expf(bound);
+  return __builtin_amdgcn_ldexpf(1.0f, min(e, 110));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, int qblocks) {
+  using V8 = typename Vec<T>::v8;
+  constexpr bool F16 = std::is_same<T, _Float16>::value;
+  const WinArgs& p = a.w;
+  __shared__ float red[16];
+  const int sub = threadIdx.x & 15, grp = threadIdx.x >> 4;
+  const bool isq = (int)blockIdx.x < qblocks;
+  int bid = isq ? blockIdx.x : blockIdx.x - qblocks;
+  const int nb = isq ? a.nq64 : a.nk64, heads = isq ? p.heads : p.kv_heads;
+  const int blk = bid % nb; bid /= nb;
+  const int h = bid % heads, b = bid / heads;
+  const int n = isq ? win_len(p.q_len, b, p.Lq) : win_len(p.kv_len, b, p.Lk);
+  float big = 0.0f;
+  for (int k = 0; k < 4; ++k) {
+    const int i = blk * 64 + k * 16 + grp;
+    float dl = 0.0f, sq = 0.0f;
+    if (i < n) {
+      const T* x = isq ? reinterpret_cast<const T*>(a.dout) + (long)b * a.do_bs + (long)h * a.do_hs + (long)i * a.do_rs
+                       : reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)h * p.v_hs + (long)i * p.v_rs;
+      const T* o = reinterpret_cast<const T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)i * p.o_rs;
+      for (int d = sub * 8; d < p.hd; d += 128) {
+        const V8 xv = ld8<T>(x + d);
+        const V8 ov = isq ? ld8<T>(o + d) : zero8<T>();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = to_f32(xv[e]);
+          dl += f * to_f32(ov[e]);
+          sq += f * f;
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) { dl += __shfl_xor(dl, s, 64); sq += __shfl_xor(sq, s, 64); }
+    if (isq && sub == 0 && i < p.Lq) {
+      const long at = ((long)b * p.heads + h) * p.Lq + i;
+      const float ls = i < n ? p.lse[at] : -__builtin_inff();
+      a.delta[at] = dl;
+      a.lse2[at] = ls == -__builtin_inff() ? __builtin_inff() : ls * 1.44269504088896340736f;
+    }
+    if (F16) big = fmaxf(big, sqrtf(sq));
+  }
+  if (!F16) return;
+  if (sub == 0) red[grp] = big;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) big = fmaxf(big, red[k]);
+    (isq ? a.domax : a.vmax)[((long)b * heads + h) * nb + blk] = big;
+  }
+}
+
+template <typename T, int HK>
+__global__ __launch_bounds__(256, HK <= 64 ? 2 : 1) void win_bwd_dkv_kernel(const WinBwdArgs a) {
+  using V8 = typename Vec<T>::v8;
+  constexpr bool F16 = std::is_same<T, _Float16>::value;
+  constexpr int QB = 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8, PT = win_pitch_tr(HK);
+  constexpr int STAGE = 2 * QB * PT + 2 * QB * 4;
+  constexpr int U = (QB * CH + 255) / 256;
+  const WinArgs& p = a.w;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+  __shared__ float sm_g[128];
+  win_lds* const lds = (win_lds*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hi = lane >> 5, l31 = lane & 31;
+
+  // block -> (batch entry, key head, key tile, query split); the longest tiles (sinks, then the first keys) come first
+  const int per = a.nst * a.sps + a.nrt * a.spr;
+  int bid = blockIdx.x;
+  const int hk = bid % p.kv_heads; bid /= p.kv_heads;
+  const int b = bid % p.batch; bid /= p.batch;
+  const bool sink = bid < a.nst * a.sps;
+  const int loc = sink ? bid : bid - a.nst * a.sps, sp = sink ? a.sps : a.spr;
+  const int tile = loc / sp, split = loc - tile * sp;
+  (void)per;
+  const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk), shift = kn - qn;
+  const int s_end = min(p.sinks, p.Lk);
+  const int ka = (sink ? 0 : s_end) + tile * BW_KEYS, kz = min(ka + BW_KEYS, sink ? s_end : p.Lk), kb = min(kz, kn);
+
+  // queries that see some key of [ka, kb)
+  int ia = 0, ib = 0;
+  if (ka < kb) {
+    ia = p.right < 0 ? 0 : win_clamp(ka - p.right - shift, 0, qn);
+    ib = p.left < 0 || sink ? qn : win_clamp(kb - 1 + p.left - shift + 1, 0, qn);
+  }
+  const int ntq = ib > ia ? (ib - ia + QB - 1) / QB : 0, its = ntq * p.group;
+  const int itb = (int)((long)its * split / sp), ite = (int)((long)its * (split + 1) / sp);
+
+  const T* K = reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hk * p.k_hs;
+  const T* V = reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hk * p.v_hs;
+  const int kw = ka + wave * 32, key = kw + l31;
+  V8 kf[NKS], vf[NKS];
+  float vsq = 0.0f;
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    const int d = ks * 16 + hi * 8;
+    const bool ok = key < kb && d < p.hd;
+    kf[ks] = ok ? ld8<T>(K + (long)key * p.k_rs + d) : zero8<T>();
+    vf[ks] = ok ? ld8<T>(V + (long)key * p.v_rs + d) : zero8<T>();
+    if (F16)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { const float f = to_f32(vf[ks][e]); vsq += f * f; }
+  }
+  float gs = 1.0f;                               // fp16: scale of dS (relative to P's) for this lane's key
+  if (F16) {
+    float dm = 0.0f;
+    const float* m = a.domax + ((long)b * p.heads + hk * p.group) * a.nq64;
+    for (int i = lane; i < p.group * a.nq64; i += 64) dm = fmaxf(dm, m[i]);
+    dm = wave_max(dm);
+    const float g = ds_scale(dm, sqrtf(win_half_sum(vsq)));
+    if (hi == 0) sm_g[wave * 32 + l31] = 1.0f / g;
+    gs = g * 0x1p-14f;
+  }
+
+  // positions that see this lane's key / that all of the wave's keys are seen from
+  const int plo = p.right < 0 ? -WIN_MAX_LEN * 2 + 1 : key - p.right, phi = p.left < 0 || sink ? WIN_MAX_LEN * 2 - 1 : key + p.left;
+  const int alo = p.right < 0 ? -WIN_MAX_LEN * 2 + 1 : kw + 31 - p.right, ahi = p.left < 0 || sink ? WIN_MAX_LEN * 2 - 1 : kw + p.left;
+  const int nlo = p.right < 0 ? -WIN_MAX_LEN * 2 + 1 : kw - p.right, nhi = p.left < 0 || sink ? WIN_MAX_LEN * 2 - 1 : kw + 31 + p.left;
+
+  V8 qr[U], gr[U];
+  float lr = 0.0f, dr = 0.0f;
+  auto load = [&](int it) {
+    const int g = it / ntq, i0 = ia + (it - g * ntq) * QB, h = hk * p.group + g, rem = ib - i0;
+    const T* qt = reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs + (long)i0 * p.q_rs;
+    const T* gt = reinterpret_cast<const T*>(a.dout) + (long)b * a.do_bs + (long)h * a.do_hs + (long)i0 * a.do_rs;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+      const bool ok = rr < rem && rr < QB && ch * 8 < p.hd;
+      qr[i] = ok ? ld8<T>(qt + (unsigned)rr * (unsigned)p.q_rs + ch * 8) : zero8<T>();
+      gr[i] = ok ? ld8<T>(gt + (unsigned)rr * (unsigned)a.do_rs + ch * 8) : zero8<T>();
+    }
+    if (tid < QB) {
+      const long at = ((long)b * p.heads + h) * p.Lq + i0 + tid;
+      lr = tid < rem ? a.lse2[at] : __builtin_inff();
+      dr = tid < rem ? a.delta[at] : 0.0f;
+    }
+  };
+  auto store = [&](int stage) {
+    win_lds* const qt = lds + stage * STAGE;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+      if (QB * CH % 256 == 0 || u < QB * CH) {
+        *(__attribute__((address_space(3))) V8*)(qt + rr * PT + ch * 16) = qr[i];
+        *(__attribute__((address_space(3))) V8*)(qt + QB * PT + rr * PT + ch * 16) = gr[i];
+      }
+    }
+    if (tid < QB) {
+      *(__attribute__((address_space(3))) float*)(qt + 2 * QB * PT + tid * 4) = lr;
+      *(__attribute__((address_space(3))) float*)(qt + 2 * QB * PT + QB * 4 + tid * 4) = dr;
+    }
+  };
+
+  f32x16 dk[NDB], dv[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dk[db][e] = dv[db][e] = 0.0f;
+  const f32x16 zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  const int rfo = l31 * PT + hi * 16, tfo = (4 * hi + ((lane & 15) >> 2)) * PT + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+  const float c = p.c;
+
+  if (itb < ite) { load(itb); store(0); }
+  if (itb + 1 < ite) load(itb + 1);
+  __syncthreads();
+  for (int it = itb; it < ite; ++it) {
+    const int cur = (it - itb) & 1;
+    if (it + 1 < ite) store(cur ^ 1);
+    if (it + 2 < ite) load(it + 2);
+    const int p0 = shift + ia + (it % ntq) * QB;           // position of the tile's first row
+    const win_lds* const qt = lds + cur * STAGE;
+    const win_lds* const gt = qt + QB * PT;
+    const win_lds* const lt = qt + 2 * QB * PT;
+    if (kw < kb && p0 + QB - 1 >= nlo && p0 <= nhi) {
+      f32x16 s = zero16, dp = zero16;
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(qt + rfo + ks * 32), kf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) dp = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(gt + rfo + ks * 32), vf[ks], dp);
+      const bool all = p0 >= alo && p0 + QB - 1 <= ahi;
+      V8 pf[2], df[2];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 ls = *(const __attribute__((address_space(3))) f32x4*)(lt + (8 * g + 4 * hi) * 4);
+        const f32x4 dl = *(const __attribute__((address_space(3))) f32x4*)(lt + QB * 4 + (8 * g + 4 * hi) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = 4 * g + e;
+          float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, (F16 ? P_EXP : 0.0f) - ls[e]));
+          if (!all) {
+            const int pe = p0 + 8 * g + 4 * hi + e;
+            pv = pe >= plo && pe <= phi ? pv : 0.0f;
+          }
+          const float ds = F16 ? pv * ((dp[x] - dl[e]) * gs) : pv * (dp[x] - dl[e]);
+          pf[x >> 3][x & 7] = from_f32<T>(pv);
+          df[x >> 3][x & 7] = from_f32<T>(ds);
+        }
+      }
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const int colb = min(db * 32 + gdh * 16, HK - 16) * 2;
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2) {
+          dv[db] = Vec<T>::mfma32(pf[h2], win_tr8<V8, PT>(gt + tfo, h2 * 16, colb), dv[db]);
+          dk[db] = Vec<T>::mfma32(df[h2], win_tr8<V8, PT>(qt + tfo, h2 * 16, colb), dk[db]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  // registers hold keys, lanes columns
+  float* part = nullptr;
+  if (sp > 1) {
+    const int tp = sink ? loc : (a.sps > 1 ? a.nst * a.sps : 0) + loc;
+    part = a.part + (((long)b * p.kv_heads + hk) * a.nparts + tp) * BW_KEYS * 2 * p.hd;
+  }
+  T* dK = reinterpret_cast<T*>(a.dk) + (long)b * a.dk_bs + (long)hk * a.dk_hs;
+  T* dV = reinterpret_cast<T*>(a.dv) + (long)b * a.dv_bs + (long)hk * a.dv_hs;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) {
+    const int d = db * 32 + l31;
+    if (d >= p.hd) continue;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int kl = wave * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi, j = ka + kl;
+      const bool live = j < kb;
+      const float gk = live ? dk[db][e] * (F16 ? sm_g[kl] * p.scale : p.scale) : 0.0f;
+      const float gv = live ? (F16 ? dv[db][e] * 0x1p-14f : dv[db][e]) : 0.0f;
+      if (part) { part[(long)kl * 2 * p.hd + d] = gk; part[(long)kl * 2 * p.hd + p.hd + d] = gv; }
+      else if (j < kz) { dK[(long)j * a.dk_rs + d] = from_f32<T>(gk); dV[(long)j * a.dv_rs + d] = from_f32<T>(gv); }
+    }
+  }
+}
+
+// dK / dV of the tiles whose query rows were split: one workgroup per tile, the parts are added in order
+template <typename T>
+__global__ __launch_bounds__(256) void win_bwd_join_kernel(const WinBwdArgs a) {
+  const WinArgs& p = a.w;
+  const int nts = a.sps > 1 ? a.nst : 0, ntr = a.spr > 1 ? a.nrt : 0;
+  int bid = blockIdx.x;
+  const int rows8 = bid % 16; bid /= 16;         // 8 keys of the tile
+  const int tt = bid % (nts + ntr); bid /= (nts + ntr);
+  const int hk = bid % p.kv_heads, b = bid / p.kv_heads;
+  const bool sink = tt < nts;
+  const int tile = sink ? tt : tt - nts, sp = sink ? a.sps : a.spr;
+  const int s_end = min(p.sinks, p.Lk);
+  const int ka = (sink ? 0 : s_end) + tile * BW_KEYS, kz = min(ka + BW_KEYS, sink ? s_end : p.Lk);
+  const int tp = sink ? tile * sp : nts * a.sps + tile * sp;
+  const float* part = a.part + (((long)b * p.kv_heads + hk) * a.nparts + tp) * BW_KEYS * 2 * p.hd;
+  T* dK = reinterpret_cast<T*>(a.dk) + (long)b * a.dk_bs + (long)hk * a.dk_hs;
+  T* dV = reinterpret_cast<T*>(a.dv) + (long)b * a.dv_bs + (long)hk * a.dv_hs;
+  const int w = 2 * p.hd;
+  for (int k = threadIdx.x; k < 8 * w; k += 256) {
+    const int kl = rows8 * 8 + k / w, d = k % w, j = ka + kl;
+    if (j >= kz) continue;
+    float s = 0.0f;
+    for (int i = 0; i < sp; ++i) s += part[(long)i * BW_KEYS * w + (long)kl * w + d];
+    if (d < p.hd) dK[(long)j * a.dk_rs + d] = from_f32<T>(s);
+    else dV[(long)j * a.dv_rs + d - p.hd] = from_f32<T>(s);
+  }
+}
+
+template <typename T, int HK>
+__global__ __launch_bounds__(256, HK <= 64 ? 2 : 1) void win_bwd_dq_kernel(const WinBwdArgs a) {
+  using V8 = typename Vec<T>::v8;
+  using V4 = typename Vec<T>::v4;
+  constexpr bool F16 = std::is_same<T, _Float16>::value;
+  constexpr int KB = 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8;
+  constexpr int PT = win_pitch_tr(HK), VP = win_pitch_row(HK), STAGE = KB * (PT + VP);
+  constexpr int U = (KB * CH + 255) / 256;
+  const WinArgs& p = a.w;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+  win_lds* const lds = (win_lds*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hi = lane >> 5, l31 = lane & 31;
+  int bid = xcd_remap(blockIdx.x, p.batch * p.heads * p.nqb);
+  const int qb = p.nqb - 1 - bid % p.nqb;
+  bid /= p.nqb;
+  const int h = bid % p.heads, b = bid / p.heads, hk = h / p.group;
+  const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk), shift = kn - qn;
+  const T* K = reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hk * p.k_hs;
+  const T* V = reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hk * p.v_hs;
+  const int i0 = qb * 128, iw = i0 + wave * 32, row = iw + l31;
+  const T* Q = reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs + (long)row * p.q_rs;
+  const T* G = reinterpret_cast<const T*>(a.dout) + (long)b * a.do_bs + (long)h * a.do_hs + (long)row * a.do_rs;
+
+  V8 qf[NKS], gf[NKS];
+  float gsq = 0.0f;
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    const int d = ks * 16 + hi * 8;
+    const bool ok = row < qn && d < p.hd;
+    qf[ks] = ok ? ld8<T>(Q + d) : zero8<T>();
+    gf[ks] = ok ? ld8<T>(G + d) : zero8<T>();
+    if (F16)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { const float f = to_f32(gf[ks][e]); gsq += f * f; }
+  }
+  const long at = ((long)b * p.heads + h) * p.Lq + row;
+  float lse = row < qn ? a.lse2[at] : __builtin_inff();
+  const float delta = row < qn ? a.delta[at] : 0.0f;
+  float undo = p.scale;
+  if (F16) {                                     // the scale of dS rides in the exponent of P
+    float vm = 0.0f;
+    const float* m = a.vmax + ((long)b * p.kv_heads + hk) * a.nk64;
+    for (int i = lane; i < a.nk64; i += 64) vm = fmaxf(vm, m[i]);
+    vm = wave_max(vm);
+    const float g = ds_scale(sqrtf(win_half_sum(gsq)), vm);
+    lse -= __builtin_amdgcn_logf(g);
+    undo = p.scale / g;
+  }
+
+  WinRange r = {0, 0, 0};
+  if (i0 < qn) r = win_range(p, shift + i0, shift + min(i0 + 127, qn - 1), kn);
+  const int n0 = (r.e0 + KB - 1) / KB, nt = n0 + (r.e1 - r.s1 + KB - 1) / KB;
+  const int pw0 = shift + iw, pw1 = shift + min(iw + 31, qn - 1), pos = shift + row;
+  const int vhi = p.right < 0 ? kn : min(kn, pos + p.right + 1), vlo = p.left < 0 ? 0 : pos - p.left;
+
+  V8 kr[U], vr[U];
+  auto load = [&](int t) {
+    const int j0 = t < n0 ? t * KB : r.s1 + (t - n0) * KB, rem = (t < n0 ? r.e0 : r.e1) - j0;
+    const T* kt = K + (long)j0 * p.k_rs;
+    const T* vt = V + (long)j0 * p.v_rs;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+      const bool ok = rr < rem && rr < KB && ch * 8 < p.hd;
+      kr[i] = ok ? ld8<T>(kt + (unsigned)rr * (unsigned)p.k_rs + ch * 8) : zero8<T>();
+      vr[i] = ok ? ld8<T>(vt + (unsigned)rr * (unsigned)p.v_rs + ch * 8) : zero8<T>();
+    }
+  };
+  auto store = [&](int stage) {
+    win_lds* const kt = lds + stage * STAGE;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+      if (KB * CH % 256 == 0 || u < KB * CH) {
+        *(__attribute__((address_space(3))) V8*)(kt + rr * PT + ch * 16) = kr[i];
+        *(__attribute__((address_space(3))) V8*)(kt + KB * PT + rr * VP + ch * 16) = vr[i];
+      }
+    }
+  };
+  f32x16 dq[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dq[db][e] = 0.0f;
+  const f32x16 zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  const int kfo = l31 * PT + hi * 16, vfo = l31 * VP + hi * 16;
+  const int tfo = (4 * hi + ((lane & 15) >> 2)) * PT + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+  const float c = p.c;
+
+  if (nt > 0) { load(0); store(0); }
+  if (nt > 1) load(1);
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    const int j0 = t < n0 ? t * KB : r.s1 + (t - n0) * KB, end = t < n0 ? r.e0 : r.e1;
+    if (t + 1 < nt) store((t + 1) & 1);
+    if (t + 2 < nt) load(t + 2);
+    const win_lds* const kt = lds + (t & 1) * STAGE;
+    const win_lds* const vt = kt + KB * PT;
+    const bool none = iw >= qn || (p.right >= 0 && j0 > pw1 + p.right) || (p.left >= 0 && j0 + KB <= pw0 - p.left && j0 >= p.sinks);
+    if (!none) {
+      f32x16 s = zero16, dp = zero16;
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(kt + kfo + ks * 32), qf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) dp = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(vt + vfo + ks * 32), gf[ks], dp);
+      const bool all = end - j0 >= KB && (p.right < 0 || j0 + KB - 1 <= pw0 + p.right) &&
+                       (p.left < 0 || j0 >= pw1 - p.left || j0 + KB <= p.sinks);
+      const int lhi = min(vhi, end);
+      V8 df[2];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lse));
+        if (!all) {
+          const int j = j0 + (e & 3) + 8 * (e >> 2) + 4 * hi;
+          pv = j < lhi && (j >= vlo || j < p.sinks) ? pv : 0.0f;
+        }
+        df[e >> 3][e & 7] = from_f32<T>(pv * (dp[e] - delta));
+      }
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const int colb = min(db * 32 + gdh * 16, HK - 16) * 2;
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2) dq[db] = Vec<T>::mfma32(win_tr8<V8, PT>(kt + tfo, h2 * 16, colb), df[h2], dq[db]);
+      }
+    }
+    __syncthreads();
+  }
+  if (row >= p.Lq) return;
+  T* O = reinterpret_cast<T*>(a.dq) + (long)b * a.dq_bs + (long)h * a.dq_hs + (long)row * a.dq_rs;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = db * 32 + 8 * g + 4 * hi;
+      if (d < p.hd) {
+        V4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(row < qn ? dq[db][4 * g + e] * undo : 0.0f);
+        *reinterpret_cast<V4*>(O + d) = w;
+      }
+    }
+}
+
+// Key tiles and query splits.  A sink tile meets every query, a tile of the rest at most left + right + 128 of them: the sinks' queries
+// are split so that their workgroups end with the others; and all are split when the tiles alone leave CUs idle.
+int64_t plan_bwd(WinBwdArgs& a) {
+  WinArgs& p = a.w;
+  p.nqb = (p.Lq + 127) / 128;
+  if (p.left < 0) p.sinks = 0;                   // everything up to the right edge is visible anyway
+  const int s_end = p.sinks < p.Lk ? p.sinks : p.Lk;
+  a.nst = (s_end + BW_KEYS - 1) / BW_KEYS;
+  a.nrt = (p.Lk - s_end + BW_KEYS - 1) / BW_KEYS;
+  a.nq64 = (p.Lq + 63) / 64;
+  a.nk64 = (p.Lk + 63) / 64;
+  const long bh = (long)p.batch * p.kv_heads;
+  long span = p.Lq;
+  if (p.left >= 0 && p.right >= 0 && (long)p.left + p.right + BW_KEYS < span) span = (long)p.left + p.right + BW_KEYS;
+  const long it_s = (long)p.group * ((p.Lq + 31) / 32), it_r = (long)p.group * ((span + 31) / 32);
+  const auto fit = [](long want, long its) { const long m = its / 4; return (int)(want < 1 || m < 1 ? 1 : (want < m ? want : m)); };
+  a.spr = a.nrt && bh * a.nrt < 256 ? fit(512 / (bh * a.nrt), it_r) : 1;
+  long ws = it_r * 2 ? (it_s * a.spr + it_r - 1) / it_r : 1;
+  if (a.nst && bh * a.nst * ws < 256 && a.nrt * bh < 256) ws = 512 / (bh * a.nst);
+  if (ws > 64) ws = 64;
+  a.sps = a.nst ? fit(ws, it_s) : 1;
+  a.nparts = (a.sps > 1 ? a.nst * a.sps : 0) + (a.spr > 1 ? a.nrt * a.spr : 0);
+  const int64_t rows = (int64_t)p.batch * p.heads * p.Lq;
+  int64_t at = 0;
+  const auto take = [&](int64_t floats) { const int64_t o = at; at += (floats + 3) / 4 * 4; return o; };
+  float* base = a.part;
+  a.delta = base + take(rows);
+  a.lse2 = base + take(rows);
+  a.domax = base + take((int64_t)p.batch * p.heads * a.nq64);
+  a.vmax = base + take(bh * a.nk64);
+  a.part = base + take(bh * a.nparts * BW_KEYS * 2 * p.hd);
+  return at * 4;
+}
+
+template <typename T, int HK>
+int launch_hk(const WinBwdArgs& a, hipStream_t st) {
+  const WinArgs& p = a.w;
+  const long tiles = (long)p.batch * p.kv_heads * (a.nst * a.sps + a.nrt * a.spr);
+  if (tiles > 0) {
+    hipLaunchKernelGGL((win_bwd_dkv_kernel<T, HK>), dim3((unsigned)tiles), dim3(256), 0, st, a);
+    HALLO_CHECK_LAUNCH();
+  }
+  if (p.Lq > 0) {
+    hipLaunchKernelGGL((win_bwd_dq_kernel<T, HK>), dim3((unsigned)(p.batch * p.heads * p.nqb)), dim3(256), 0, st, a);
+    HALLO_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+template <typename T>
+int launch(const WinBwdArgs& a, hipStream_t st) {
+  const WinArgs& p = a.w;
+  const bool f16 = std::is_same<T, _Float16>::value;
+  const long qblocks = (long)p.batch * p.heads * a.nq64, kblocks = f16 ? (long)p.batch * p.kv_heads * a.nk64 : 0;
+  if (qblocks + kblocks > 0) {
+    hipLaunchKernelGGL((win_bwd_prep_kernel<T>), dim3((unsigned)(qblocks + kblocks)), dim3(256), 0, st, a, (int)qblocks);
+    HALLO_CHECK_LAUNCH();
+  }
+  int rc;
+  switch ((p.hd + 15) / 16) {
+    case 1: rc = launch_hk<T, 16>(a, st); break;
+    case 2: rc = launch_hk<T, 32>(a, st); break;
+    case 3: rc = launch_hk<T, 48>(a, st); break;
+    case 4: rc = launch_hk<T, 64>(a, st); break;
+    case 5: rc = launch_hk<T, 80>(a, st); break;
+    case 6: rc = launch_hk<T, 96>(a, st); break;
+    case 7: rc = launch_hk<T, 112>(a, st); break;
+    case 8: rc = launch_hk<T, 128>(a, st); break;
+    case 9: rc = launch_hk<T, 144>(a, st); break;
+    default: rc = launch_hk<T, 160>(a, st);
+  }
+  if (rc) return rc;
+  const long nj = (long)p.batch * p.kv_heads * ((a.sps > 1 ? a.nst : 0) + (a.spr > 1 ? a.nrt : 0)) * 16;
+  if (nj > 0) {
+    hipLaunchKernelGGL((win_bwd_join_kernel<T>), dim3((unsigned)nj), dim3(256), 0, st, a);
+    HALLO_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+bool bwd_args(const hallo_window_attn_bwd_desc* d, WinBwdArgs& a) {
+  a = WinBwdArgs{};
+  if (!d || !win_args(&d->fwd, a.w)) return false;
+  const int64_t strides[] = {d->do_bs, d->do_rs, d->do_hs, d->dq_bs, d->dq_rs, d->dq_hs, d->dk_bs, d->dk_rs, d->dk_hs, d->dv_bs, d->dv_rs, d->dv_hs};
+  for (int64_t s : strides)
+    if (s < 0 || s % 8) return false;
+  const int64_t row_strides[] = {d->do_rs, d->dq_rs, d->dk_rs, d->dv_rs};
+  for (int64_t s : row_strides)
+    if (s > WIN_MAX_STRIDE) return false;
+  const void* ptrs[] = {d->dout, d->dq, d->dk, d->dv};
+  for (const void* q : ptrs)
+    if (reinterpret_cast<uintptr_t>(q) & 15) return false;
+  a.dout = d->dout; a.dq = d->dq; a.dk = d->dk; a.dv = d->dv;
+  a.do_bs = d->do_bs; a.do_rs = d->do_rs; a.do_hs = d->do_hs; a.dq_bs = d->dq_bs; a.dq_rs = d->dq_rs; a.dq_hs = d->dq_hs;
+  a.dk_bs = d->dk_bs; a.dk_rs = d->dk_rs; a.dk_hs = d->dk_hs; a.dv_bs = d->dv_bs; a.dv_rs = d->dv_rs; a.dv_hs = d->dv_hs;
+  return true;
+}
+
+}  // namespace
+}  // namespace hallo
+
+extern "C" int64_t hallo_window_attention_backward_workspace(const hallo_window_attn_bwd_desc* d) {
+  using namespace hallo;
+  WinBwdArgs a;
+  if (!bwd_args(d, a)) return -22;
+  if (a.w.batch == 0) return 0;
+  return plan_bwd(a);
+}
+
+extern "C" int hallo_window_attention_backward(const hallo_window_attn_bwd_desc* d, void* stream) {
+  using namespace hallo;
+  WinBwdArgs a;
+  if (!bwd_args(d, a)) return -22;
+  const WinArgs& p = a.w;
+  if (p.batch == 0 || (p.Lq == 0 && p.Lk == 0)) return 0;
+  if (p.Lq > 0 && (!p.q || !p.o || !p.lse || !a.dout || !a.dq)) return -22;
+  if (p.Lk > 0 && (!p.k || !p.v || !a.dk || !a.dv)) return -22;
+  const int64_t need = hallo_window_attention_backward_workspace(d);
+  if (need > 0 && (!d->fwd.workspace || d->fwd.workspace_bytes < need || (reinterpret_cast<uintptr_t>(d->fwd.workspace) & 15))) return -22;
+  a.part = (float*)d->fwd.workspace;
+  plan_bwd(a);
+  if ((int64_t)p.batch * p.kv_heads * ((int64_t)a.nst * a.sps + (int64_t)a.nrt * a.spr) * 16 > 0x7fffffff) return -22;
+  return d->fwd.dtype == DT_F16 ? launch<_Float16>(a, (hipStream_t)stream) : launch<__bf16>(a, (hipStream_t)stream);
+}

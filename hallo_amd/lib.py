@@ -101,6 +101,41 @@ class AttnDesc(C.Structure):
     ]
 
 
+class RopeDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("y", C.c_void_p),
+        ("x_bs", C.c_int64), ("x_rs", C.c_int64), ("y_bs", C.c_int64), ("y_rs", C.c_int64),
+        ("freq", C.c_void_p), ("pos", C.c_void_p), ("pos_bs", C.c_int64),
+        ("batch", C.c_int64), ("L", C.c_int64),
+        ("heads", C.c_int), ("head_dim", C.c_int), ("n_axes", C.c_int),
+        ("dims", C.c_int * 4), ("grid", C.c_int * 4), ("origin", C.c_int * 4),
+        ("interleaved", C.c_int), ("inverse", C.c_int), ("dtype", C.c_int),
+    ]
+
+
+class WindowAttnDesc(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
+        ("q_bs", C.c_int64), ("q_rs", C.c_int64), ("q_hs", C.c_int64), ("k_bs", C.c_int64), ("k_rs", C.c_int64), ("k_hs", C.c_int64),
+        ("v_bs", C.c_int64), ("v_rs", C.c_int64), ("v_hs", C.c_int64), ("o_bs", C.c_int64), ("o_rs", C.c_int64), ("o_hs", C.c_int64),
+        ("q_len", C.c_void_p), ("kv_len", C.c_void_p),
+        ("Lq", C.c_int64), ("Lk", C.c_int64),
+        ("batch", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+        ("left", C.c_int), ("right", C.c_int), ("sinks", C.c_int),
+        ("scale", C.c_float), ("dtype", C.c_int),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class WindowAttnBwdDesc(C.Structure):
+    _fields_ = [
+        ("fwd", WindowAttnDesc),
+        ("dout", C.c_void_p), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("do_bs", C.c_int64), ("do_rs", C.c_int64), ("do_hs", C.c_int64), ("dq_bs", C.c_int64), ("dq_rs", C.c_int64), ("dq_hs", C.c_int64),
+        ("dk_bs", C.c_int64), ("dk_rs", C.c_int64), ("dk_hs", C.c_int64), ("dv_bs", C.c_int64), ("dv_rs", C.c_int64), ("dv_hs", C.c_int64),
+    ]
+
+
 # symbol -> (restype, argtypes); every symbol include/hallo_amd.h declares is listed here and
 # tests/test_abi.py checks that the built library exports each of them.
 SYMBOLS = {
@@ -148,6 +183,17 @@ SYMBOLS = {
     "hallo_w2v_conv0_gn_gelu": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                          C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, C.c_void_p]),
     "hallo_lerp_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "hallo_layernorm_train": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                        C.c_int64, C.c_int, C.c_float, C.c_int, C.c_void_p]),
+    "hallo_layernorm_backward_workspace": (C.c_int64, [C.c_int64, C.c_int]),
+    "hallo_layernorm_backward": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                           C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_int,
+                                           C.c_void_p]),
+    "hallo_rope": (C.c_int, [C.POINTER(RopeDesc), C.c_void_p]),
+    "hallo_window_attention_workspace": (C.c_int64, [C.POINTER(WindowAttnDesc)]),
+    "hallo_window_attention": (C.c_int, [C.POINTER(WindowAttnDesc), C.c_void_p]),
+    "hallo_window_attention_backward_workspace": (C.c_int64, [C.POINTER(WindowAttnBwdDesc)]),
+    "hallo_window_attention_backward": (C.c_int, [C.POINTER(WindowAttnBwdDesc), C.c_void_p]),
     "hallo_timestep_embedding": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "hallo_cfg_ddim_step": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int,
                                       C.c_int, C.c_float, C.c_float, C.c_float, C.c_int, C.c_void_p]),

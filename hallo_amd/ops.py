@@ -5,6 +5,7 @@ stream; every computation goes through the hand-written gfx950 kernels.  Activat
 token-major: [frames, H*W, C] with C contiguous.
 """
 import ctypes as C
+import math
 import threading
 
 import torch
@@ -851,3 +852,292 @@ def lerp_rows(x, out_rows):
     _l.check(_l.load().hallo_lerp_rows(_p(x), _p(out), x.shape[0], out_rows, x.shape[1], dtype_code(x.dtype), _stream()),
              "hallo_lerp_rows")
     return out
+
+
+# ---- transformer-block operators with gradients: LayerNorm, rotary positions, window attention -------------------------------------
+# Their workspaces are allocated per call: a captured graph gets them from its own pool, so two graphs never share one, and the
+# allocator orders the reuse of a freed one on its stream.
+
+class _on:
+    """The stream to launch on for tensors of `t`'s device -- that device's current stream, with the device made current for the
+    launch when another one is (a stream only takes launches from its own device)."""
+
+    def __init__(self, t):
+        self.device = t.device
+        self._guard = None
+
+    def __enter__(self):
+        if self.device.index != torch.cuda.current_device():
+            self._guard = torch.cuda.device(self.device)
+            self._guard.__enter__()
+        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+        return False
+
+
+def _need(ok, what):
+    if not ok:
+        raise _l.HalloLibraryError(what)
+
+
+def _same(name, t, like, dtype=None):
+    """`t` is on `like`'s device and of its type (or `dtype`)."""
+    _need(t.device == like.device, f"{name} is on {t.device}, expected {like.device}")
+    _need(t.dtype == (dtype or like.dtype), f"{name} is {t.dtype}, expected {dtype or like.dtype}")
+
+
+def _rows2d(name, x):
+    """x [..., C] as (rows, C, row pitch): contiguous, or a 2-D view with contiguous rows."""
+    _need(x.dim() >= 1 and x.shape[-1] >= 1, f"{name}: expected [..., C] with C >= 1, got {tuple(x.shape)}")
+    Cd = x.shape[-1]
+    if x.is_contiguous() or x.numel() == 0:
+        return x.numel() // Cd, Cd, Cd
+    _need(x.dim() == 2 and (x.stride(1) == 1 or Cd == 1) and (x.stride(0) >= Cd or x.shape[0] == 1),
+          f"{name}: expected a contiguous tensor or a 2-D view with contiguous rows, got shape {tuple(x.shape)} strides {x.stride()}")
+    return x.shape[0], Cd, max(x.stride(0), Cd)
+
+
+def _affine(x, gamma, beta):
+    """Checks gamma / beta [C] (x's type or fp32, the same for both); returns the library's affine_f32 flag."""
+    ws = [w for w in (gamma, beta) if w is not None]
+    for name, w in (("gamma", gamma), ("beta", beta)):
+        if w is not None:
+            _need(w.device == x.device and w.dtype in (x.dtype, torch.float32) and w.is_contiguous() and w.numel() == x.shape[-1],
+                  f"{name}: expected [{x.shape[-1]}] of {x.dtype} or float32 on {x.device}, got {tuple(w.shape)} {w.dtype} on {w.device}")
+    _need(len({w.dtype for w in ws}) <= 1, "gamma and beta have different types")
+    return 1 if ws and ws[0].dtype == torch.float32 else 0
+
+
+def layernorm_train(x, gamma=None, beta=None, eps=1e-5, *, out=None):
+    """(y, stats): y = LayerNorm(x [..., C]) * gamma + beta and the row statistics fp32 [rows, 2] = (mean, rstd) that
+    layernorm_backward() takes.  Any C up to 16384.  gamma / beta: [C] of x's type or fp32 (master weights), or None.  out may be x."""
+    _chk_dev(x, gamma, beta, out)
+    code = dtype_code(x.dtype)
+    rows, Cd, ldx = _rows2d("x", x)
+    f32 = _affine(x, gamma, beta)
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    _same("out", out, x)
+    _need(out.shape == x.shape, f"out: expected {tuple(x.shape)}, got {tuple(out.shape)}")
+    ldy = _rows2d("out", out)[2]
+    stats = torch.empty((rows, 2), device=x.device, dtype=torch.float32)
+    with _on(x) as st:
+        _l.check(_l.load().hallo_layernorm_train(_p(x), ldx, _p(out), ldy, _p(gamma), _p(beta), f32, _p(stats), rows, Cd, float(eps), code,
+                                                 st), "hallo_layernorm_train")
+    return out, stats
+
+
+def layernorm_backward(dy, x, stats, gamma=None, *, weight_grads=True, out=None):
+    """(dx, dgamma, dbeta) of layernorm_train(x, gamma, ...) for dy; stats as it returned them.  dgamma / dbeta are fp32 [C] (None with
+    weight_grads=False: frozen weights).  out (for dx) may be dy.  Results repeat bit for bit."""
+    _chk_dev(dy, x, stats, gamma, out)
+    code = dtype_code(x.dtype)
+    rows, Cd, ldx = _rows2d("x", x)
+    _same("dy", dy, x)
+    _need(dy.shape == x.shape, f"dy: expected {tuple(x.shape)}, got {tuple(dy.shape)}")
+    ldd = _rows2d("dy", dy)[2]
+    _same("stats", stats, x, torch.float32)
+    _need(stats.is_contiguous() and stats.shape == (rows, 2), f"stats: expected contiguous ({rows}, 2), got {tuple(stats.shape)}")
+    f32 = _affine(x, gamma, None)
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    _same("out", out, x)
+    _need(out.shape == x.shape, f"out: expected {tuple(x.shape)}, got {tuple(out.shape)}")
+    ldo = _rows2d("out", out)[2]
+    lib = _l.load()
+    wg = ws = None
+    need = 0
+    if weight_grads:
+        wg = torch.empty((2, Cd), device=x.device, dtype=torch.float32)
+        need = lib.hallo_layernorm_backward_workspace(rows, Cd)
+        _need(need >= 0, f"hallo_layernorm_backward_workspace({rows}, {Cd}) failed with status {need}")
+        ws = torch.empty(max(need // 4, 1), device=x.device, dtype=torch.float32)
+    with _on(x) as st:
+        _l.check(lib.hallo_layernorm_backward(_p(dy), ldd, _p(x), ldx, _p(stats), _p(gamma), f32, _p(out), ldo,
+                                              _p(wg[0]) if weight_grads else None, _p(wg[1]) if weight_grads else None, _p(ws), need, rows,
+                                              Cd, code, st), "hallo_layernorm_backward")
+    return (out, wg[0], wg[1]) if weight_grads else (out, None, None)
+
+
+class RopeAxes:
+    """Rotary frequencies of up to four position axes: dims[a] (even) columns of every head for axis a, pair i of them turning by
+    position * theta^(-2i / dims[a]).  Built once, on the host, and usable from any stream (not inside a graph capture)."""
+    __slots__ = ("dims", "head_dim", "theta", "interleaved", "freq")
+
+    def __init__(self, dims, head_dim, theta=10000.0, interleaved=False, device="cuda"):
+        dims = tuple(int(d) for d in dims)
+        _need(1 <= len(dims) <= 4 and all(d >= 2 and d % 2 == 0 for d in dims), f"dims: expected 1 to 4 even widths, got {dims}")
+        _need(head_dim % 2 == 0 and 2 <= head_dim <= 256 and sum(dims) <= head_dim, f"dims {dims} do not fit head_dim {head_dim} (even, at most 256)")
+        _need(theta > 0 and math.isfinite(theta), f"theta: expected a positive number, got {theta}")
+        self.dims, self.head_dim, self.theta, self.interleaved = dims, int(head_dim), float(theta), bool(interleaved)
+        turns = [int(round(self.theta ** (-2.0 * i / d) / (2.0 * math.pi) * 2.0 ** 64)) % (1 << 64) for d in dims for i in range(d // 2)]
+        self.freq = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64).to(device)
+
+
+def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
+    """Rotary positions on x [B, L, heads * head_dim] (any batch / row stride: column slices of a fused q|k|v buffer, q|k together).
+
+    Positions: pos int32 [L, axes] or [B, L, axes]; or grid = the axes' lengths with L cells, the last axis fastest, counted from
+    `origin` (default 0).  inverse=True turns back: the gradient with respect to x of rope(x) is rope(dy, inverse=True).  out may be x."""
+    _chk_dev(x, pos, out, axes.freq)
+    code = dtype_code(x.dtype)
+    n = len(axes.dims)
+    _need(x.dim() == 3 and x.shape[2] % axes.head_dim == 0 and x.shape[2] > 0 and x.stride(2) == 1,
+          f"x: expected [B, L, heads * {axes.head_dim}] with contiguous columns, got {tuple(x.shape)} strides {x.stride()}")
+    _need(axes.freq.device == x.device, f"axes were built on {axes.freq.device}, x is on {x.device}")
+    B, L, W = x.shape
+    if out is None:
+        out = torch.empty((B, L, W), device=x.device, dtype=x.dtype)
+    _same("out", out, x)
+    _need(out.shape == x.shape and out.stride(2) == 1 and (L <= 1 or out.stride(1) >= W) and (B <= 1 or L == 0 or out.stride(0) > 0),
+          f"out: expected {tuple(x.shape)} with rows that do not overlap, got {tuple(out.shape)} strides {out.stride()}")
+    _need((pos is None) != (grid is None), "give either pos or grid")
+    d = _l.RopeDesc()
+    d.x, d.y = x.data_ptr(), out.data_ptr()
+    d.x_bs, d.x_rs = (x.stride(0) if B > 1 else 0), (x.stride(1) if L > 1 else W)
+    d.y_bs, d.y_rs = (out.stride(0) if B > 1 else 0), (out.stride(1) if L > 1 else W)
+    d.freq = axes.freq.data_ptr()
+    if pos is not None:
+        _need(origin is None, "origin goes with grid")
+        _same("pos", pos, x, torch.int32)
+        _need(pos.is_contiguous() and tuple(pos.shape) in ((L, n), (B, L, n)), f"pos: expected contiguous ({L}, {n}) or ({B}, {L}, {n}), got {tuple(pos.shape)}")
+        d.pos, d.pos_bs = pos.data_ptr(), (L * n if pos.dim() == 3 else 0)
+    else:
+        grid, origin = tuple(grid), tuple(origin) if origin is not None else (0,) * n
+        _need(len(grid) == n and len(origin) == n and all(g >= 1 for g in grid) and math.prod(grid) == L,
+              f"grid {grid} (origin {origin}): expected {n} lengths with {L} cells")
+        _need(all(-2 ** 31 <= o and o + g <= 2 ** 31 for o, g in zip(origin, grid)), f"positions from {origin} on pass 32 bits")
+        for i in range(n):
+            d.grid[i], d.origin[i] = grid[i], origin[i]
+        d.pos, d.pos_bs = None, 0
+    for i in range(n):
+        d.dims[i] = axes.dims[i]
+    d.batch, d.L, d.heads, d.head_dim, d.n_axes = B, L, W // axes.head_dim, axes.head_dim, n
+    d.interleaved, d.inverse, d.dtype = int(axes.interleaved), int(bool(inverse)), code
+    with _on(x) as st:
+        _l.check(_l.load().hallo_rope(C.byref(d), st), "hallo_rope")
+    return out
+
+
+def _heads4(name, t, heads, hd):
+    """[B, L, heads * hd] or [B, L, heads, hd] view -> its (batch, row, head) strides."""
+    if t.dim() == 3:
+        _need(t.shape[2] == heads * hd, f"{name}: expected [B, L, {heads} * {hd}], got {tuple(t.shape)}")
+        st = (t.stride(0), t.stride(1), hd)
+    else:
+        _need(t.dim() == 4 and t.shape[2] == heads and t.shape[3] == hd, f"{name}: expected [B, L, {heads}, {hd}], got {tuple(t.shape)}")
+        st = (t.stride(0), t.stride(1), t.stride(2))
+    # strides of single or absent rows, entries and heads never count
+    st = [0 if t.shape[0] <= 1 else st[0], 0 if t.shape[1] <= 1 else st[1], hd if heads == 1 else st[2]]
+    _need(t.stride(-1) == 1 and all(s % 8 == 0 for s in st) and st[1] <= 1 << 24 and (t.data_ptr() % 16 == 0 or t.numel() == 0),
+          f"{name}: expected contiguous head rows, strides that are multiples of 8 (rows at most 2^24 apart) and a 16-byte aligned start, "
+          f"got strides {t.stride()}")
+    return st
+
+
+def _writable(name, t, st):
+    _need(all(s > 0 or n <= 1 for s, n in zip(st, t.shape[:2])) and st[2] > 0, f"{name}: overlapping rows, strides {t.stride()}")
+    return st
+
+
+def _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale):
+    code = dtype_code(q.dtype)
+    _need(heads >= 1, f"heads: {heads}")
+    kv_heads = heads if kv_heads is None else kv_heads
+    _need(kv_heads >= 1 and heads % kv_heads == 0, f"{heads} query heads do not share {kv_heads} key heads")
+    _need(q.dim() in (3, 4) and q.shape[-1] >= 1 and (q.dim() == 4 or q.shape[2] % heads == 0), f"q: expected [B, L, {heads} * head_dim] or 4-D, got {tuple(q.shape)}")
+    hd = q.shape[3] if q.dim() == 4 else q.shape[2] // heads
+    _need(hd % 8 == 0 and 8 <= hd <= 160, f"head_dim {hd}: expected a multiple of 8 up to 160")
+    B, Lq, Lk = q.shape[0], q.shape[1], k.shape[1]
+    _need(Lq <= 1 << 29 and Lk <= 1 << 29, f"lengths {Lq}, {Lk}: at most 2^29")
+    for name, t in (("k", k), ("v", v)):
+        _same(name, t, q)
+        _need(t.dim() in (3, 4) and t.shape[0] == B and t.shape[1] == Lk, f"{name}: expected [{B}, {Lk}, ...], got {tuple(t.shape)}")
+    for name, t in (("q_len", q_len), ("kv_len", kv_len)):
+        if t is not None:
+            _same(name, t, q, torch.int32)
+            _need(t.is_contiguous() and t.shape == (B,), f"{name}: expected contiguous ({B},), got {tuple(t.shape)}")
+    _need(sinks >= 0, f"sinks: {sinks}")
+    scale = hd ** -0.5 if scale is None else float(scale)
+    _need(0.0 < scale < 1e30, f"scale: expected a positive number, got {scale}")
+    d = _l.WindowAttnDesc()
+    d.q, d.k, d.v, d.o, d.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), (lse.data_ptr() if lse is not None else None)
+    d.q_bs, d.q_rs, d.q_hs = _heads4("q", q, heads, hd)
+    d.k_bs, d.k_rs, d.k_hs = _heads4("k", k, kv_heads, hd)
+    d.v_bs, d.v_rs, d.v_hs = _heads4("v", v, kv_heads, hd)
+    d.o_bs, d.o_rs, d.o_hs = _heads4("o", o, heads, hd)
+    d.q_len, d.kv_len = (t.data_ptr() if t is not None else None for t in (q_len, kv_len))
+    d.Lq, d.Lk, d.batch, d.heads, d.kv_heads, d.head_dim = Lq, Lk, B, heads, kv_heads, hd
+    edge = lambda n: -1 if n < 0 else min(int(n), 1 << 29)
+    d.left, d.right, d.sinks, d.scale, d.dtype = edge(left), edge(right), edge(sinks), scale, code
+    d.workspace, d.workspace_bytes = None, 0
+    return d, kv_heads, hd
+
+
+def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0, q_len=None, kv_len=None, scale=None, out=None,
+                     return_lse=False):
+    """softmax(scale q k^T) v over a sliding window and `sinks` always-visible first keys.
+
+    q [B, Lq, heads * head_dim], k / v [B, Lk, kv_heads * head_dim] (or 4-D [B, L, heads, head_dim] views in any order of memory); query
+    head h reads key head h // (heads // kv_heads).  Query i stands at p = kv_len - q_len + i and sees key j iff j < kv_len,
+    j <= p + right, and j >= p - left or j < sinks; a negative left / right means no limit, so the default is causal attention with the
+    queries at the end of the keys -- a prompt, a chunk of new tokens, or one new token against a cache of capacity Lk.  q_len / kv_len:
+    int32 [B] on the device (default Lq / Lk), clamped to the tensors' lengths.  Queries that see nothing or are padding get zeros.
+    Keys behind kv_len, or outside of every window, may hold anything.  head_dim: a multiple of 8 up to 160.
+
+    return_lse: (out, lse), lse fp32 [B, heads, Lq] (-inf where nothing is visible), as window_attention_backward() takes it."""
+    _chk_dev(q, k, v, q_len, kv_len, out)
+    if out is None:
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    _same("out", out, q)
+    _need(out.shape == q.shape, f"out: expected {tuple(q.shape)}, got {tuple(out.shape)}")
+    lse = torch.empty((q.shape[0], heads, q.shape[1]), device=q.device, dtype=torch.float32) if return_lse else None
+    d, _, hd = _window_desc(q, k, v, out, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale)
+    _writable("out", out, (d.o_bs, d.o_rs, d.o_hs))
+    lib = _l.load()
+    need = lib.hallo_window_attention_workspace(C.byref(d))
+    _need(need >= 0, f"hallo_window_attention_workspace failed with status {need}")
+    if need:
+        ws = torch.empty(need // 4, device=q.device, dtype=torch.float32)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    with _on(q) as st:
+        _l.check(lib.hallo_window_attention(C.byref(d), st), "hallo_window_attention")
+    return (out, lse) if return_lse else out
+
+
+def window_attention_backward(do, q, k, v, o, lse, heads, *, kv_heads=None, left=-1, right=0, sinks=0, q_len=None, kv_len=None, scale=None,
+                              dq=None, dk=None, dv=None):
+    """(dq, dk, dv) of o, lse = window_attention(q, k, v, ..., return_lse=True) for do, with the same arguments.  dk / dv are summed over
+    the query heads that share a key head; padded rows get zeros.  Results repeat bit for bit."""
+    _chk_dev(do, q, k, v, o, lse, q_len, kv_len, dq, dk, dv)
+    _same("o", o, q)
+    _same("do", do, q)
+    _same("lse", lse, q, torch.float32)
+    _need(o.shape == q.shape and do.shape == q.shape, f"o, do: expected {tuple(q.shape)}, got {tuple(o.shape)}, {tuple(do.shape)}")
+    _need(lse.is_contiguous() and lse.shape == (q.shape[0], heads, q.shape[1]), f"lse: expected contiguous ({q.shape[0]}, {heads}, {q.shape[1]}), got {tuple(lse.shape)}")
+    w, kv_heads, hd = _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale)
+    d = _l.WindowAttnBwdDesc()
+    d.fwd = w
+    outs = []
+    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if t is None:
+            t = torch.empty(like.shape, device=q.device, dtype=q.dtype)
+        _same(name, t, q)
+        _need(t.shape == like.shape, f"{name}: expected {tuple(like.shape)}, got {tuple(t.shape)}")
+        outs.append(t)
+    d.dout, d.dq, d.dk, d.dv = do.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), outs[2].data_ptr()
+    d.do_bs, d.do_rs, d.do_hs = _heads4("do", do, heads, hd)
+    d.dq_bs, d.dq_rs, d.dq_hs = _writable("dq", outs[0], _heads4("dq", outs[0], heads, hd))
+    d.dk_bs, d.dk_rs, d.dk_hs = _writable("dk", outs[1], _heads4("dk", outs[1], kv_heads, hd))
+    d.dv_bs, d.dv_rs, d.dv_hs = _writable("dv", outs[2], _heads4("dv", outs[2], kv_heads, hd))
+    lib = _l.load()
+    need = lib.hallo_window_attention_backward_workspace(C.byref(d))
+    _need(need >= 0, f"hallo_window_attention_backward_workspace failed with status {need}")
+    ws = torch.empty(max(need // 4, 4), device=q.device, dtype=torch.float32)
+    d.fwd.workspace, d.fwd.workspace_bytes = ws.data_ptr(), need
+    with _on(q) as st:
+        _l.check(lib.hallo_window_attention_backward(C.byref(d), st), "hallo_window_attention_backward")
+    return tuple(outs)

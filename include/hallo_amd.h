@@ -422,6 +422,81 @@ int hallo_w2v_conv0_gn_gelu(const float* wave, int64_t n_samples, const float* w
                             void* y, float* workspace, int C, int k, int stride, float eps, int dtype, void* stream);
 int hallo_lerp_rows(const void* x, void* y, int in_rows, int out_rows, int C, int dtype, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * LayerNorm for training.  x [rows, C] (row pitch ldx >= C elements, any C in 1 .. 16384, any alignment), stats fp32 [rows][2] =
+ * (mean, rstd).  gamma / beta [C] in `dtype`, or fp32 with affine_f32 = 1; null = 1 / 0.
+ * hallo_layernorm_train:    y = (x - mean) * rstd * gamma + beta, and stats.  y may be x.
+ * hallo_layernorm_backward: with xh = (x - mean) * rstd and g = dy * gamma
+ *   dx = rstd * (g - mean_C(g) - xh * mean_C(g * xh)),  dgamma[c] = sum_rows(dy * xh),  dbeta[c] = sum_rows(dy)
+ *   dgamma / dbeta are fp32 [C]; both null: only dx.  dx may be dy.  workspace: hallo_layernorm_backward_workspace(rows, C) bytes
+ *   (needed with dgamma).  Sums run in a fixed order: results repeat bit for bit.
+ */
+int hallo_layernorm_train(const void* x, int64_t ldx, void* y, int64_t ldy, const void* gamma, const void* beta, int affine_f32,
+                          float* stats, int64_t rows, int C, float eps, int dtype, void* stream);
+int64_t hallo_layernorm_backward_workspace(int64_t rows, int C);
+int hallo_layernorm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* stats, const void* gamma,
+                             int affine_f32, void* dx, int64_t lddx, float* dgamma, float* dbeta, void* workspace,
+                             int64_t workspace_bytes, int64_t rows, int C, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * hallo_rope: rotary positions over 1 .. 4 axes on x [batch, L, heads * head_dim] (batch / row strides in elements).  Axis a owns the
+ * dims[a] (even) columns of every head behind those of the axes before it; its pair i turns by position_a * freq, freq[pair] being a
+ * fraction of a turn times 2^64 (axes concatenated, dims[a] / 2 each).  Pairs are (2i, 2i + 1) with interleaved = 1, else
+ * (i, i + dims[a] / 2).  Columns behind the last axis are copied.  head_dim even, at most 256.
+ * Positions: pos int32 [batch or 1, L, n_axes] (pos_bs = 0: one row for all entries), or pos = null and a grid whose cells are the L
+ * tokens, the last axis fastest, counted from origin.  inverse = 1: negative angles, which is the gradient.  y may be x (same strides).
+ */
+typedef struct hallo_rope_desc {
+  const void* x; void* y;
+  int64_t x_bs, x_rs, y_bs, y_rs;
+  const uint64_t* freq;
+  const int* pos;
+  int64_t pos_bs;
+  int64_t batch, L;
+  int heads, head_dim, n_axes;
+  int dims[4], grid[4], origin[4];
+  int interleaved, inverse, dtype;
+} hallo_rope_desc;
+int hallo_rope(const hallo_rope_desc* d, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * hallo_window_attention: softmax(scale q k^T) v over a sliding window and always-visible first keys.  Query i of entry b stands at
+ * p = kv_len[b] - q_len[b] + i and sees key j iff j < kv_len[b], j <= p + right (right < 0: no limit), and j >= p - left (left < 0: no
+ * limit) or j < sinks.  q [batch, Lq, heads, head_dim], k / v [batch, Lk, kv_heads, head_dim] with heads % kv_heads == 0 (query head h
+ * reads key head h / (heads / kv_heads)), o like q; strides in elements, multiples of 8, row strides at most 2^24, 16-byte aligned bases;
+ * head_dim % 8 == 0, at most 160; lengths at most 2^29.
+ * q_len / kv_len: int32 [batch] on the device, clamped to 0 .. Lq / Lk; null = Lq / Lk.  A query that sees nothing, and one at or behind
+ * q_len, gets zeros and lse = -inf.  lse (may be null): fp32 [batch, heads, Lq], natural logarithm of the row's sum.
+ * What lies at or behind kv_len, or outside of every query's window, is not used and may hold anything.
+ * workspace: hallo_window_attention_workspace(d) bytes, 0 unless the keys are split over workgroups.
+ *
+ * hallo_window_attention_backward: dq, dk, dv for dout, with q, k, v, o, lse and the mask as in `fwd` (fwd.o and fwd.lse are read; lse
+ * must be there).  dk / dv are summed over the query heads of a key head; rows at or behind q_len / kv_len are written as zeros.
+ * Deterministic.  fwd.workspace: hallo_window_attention_backward_workspace(d) bytes.
+ */
+typedef struct hallo_window_attn_desc {
+  const void* q; const void* k; const void* v; void* o;
+  float* lse;
+  int64_t q_bs, q_rs, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, o_bs, o_rs, o_hs;
+  const int* q_len; const int* kv_len;
+  int64_t Lq, Lk;
+  int batch, heads, kv_heads, head_dim;
+  int left, right, sinks;
+  float scale;
+  int dtype;
+  void* workspace;
+  int64_t workspace_bytes;
+} hallo_window_attn_desc;
+typedef struct hallo_window_attn_bwd_desc {
+  hallo_window_attn_desc fwd;
+  const void* dout; void* dq; void* dk; void* dv;
+  int64_t do_bs, do_rs, do_hs, dq_bs, dq_rs, dq_hs, dk_bs, dk_rs, dk_hs, dv_bs, dv_rs, dv_hs;
+} hallo_window_attn_bwd_desc;
+int64_t hallo_window_attention_workspace(const hallo_window_attn_desc* d);
+int hallo_window_attention(const hallo_window_attn_desc* d, void* stream);
+int64_t hallo_window_attention_backward_workspace(const hallo_window_attn_bwd_desc* d);
+int hallo_window_attention_backward(const hallo_window_attn_bwd_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
