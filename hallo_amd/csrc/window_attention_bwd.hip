@@ -4,8 +4,8 @@
 //   dV = P^T dO,   dS = P * (dO V^T - delta),   dQ = scale dS K,   dK = scale dS^T Q
 // summed over the query heads that share a key head.  Three launches, four with split keys:
 //   prep   delta and lse * log2(e) of every query (fp32; +inf where a query has no visible key, so its P is 0)
-//   dkv    a workgroup owns 128 keys (a wave 32): K and V stay in registers as MFMA operands, dK and dV as accumulators, and the query
-//          rows that see the keys stream through LDS, for all heads of the group -- shared heads need no atomics
+//   dkv    a workgroup owns 128 keys: K and V stay in registers as MFMA operands, dK and dV as accumulators, and the query rows that see
+//          the keys stream through LDS, for all heads of the group -- shared heads need no atomics
 //   dq     a workgroup owns 128 queries of a head (a wave 32), the visible keys stream through LDS
 //   join   the sinks are seen by every query: their key tiles' query rows are split over workgroups, fp32 parts are added here in order
 //          (also used for all keys when there are too few key tiles to fill the chip)
@@ -100,29 +100,36 @@ __global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, i
   }
 }
 
+// Eight waves: four groups of 32 keys times two roles, so that a wave keeps ONE operand and ONE accumulator (HK = 128: 32 + 64
+// registers; both in one wave are 400 registers, and hipcc then moves 128 accumulators between its two register files in every tile) and a
+// SIMD has a wave of each role, whose matrix and vector work overlap.
+//   role 0, tile t:      S = Q K^T, P = exp2(S c - lse2), dV += P^T dO; leaves P (storage type) for its partner in LDS
+//   role 1, tile t - 1:  dP = dO V^T, dS = P * (dP - delta), dK += dS^T Q
+// Q and dO tiles are kept for two iterations (three LDS stages), P in two, so one barrier per tile is enough.
 template <typename T, int HK>
-__global__ __launch_bounds__(256, HK <= 64 ? 2 : 1) void win_bwd_dkv_kernel(const WinBwdArgs a) {
+__global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(const WinBwdArgs a) {
   using V8 = typename Vec<T>::v8;
   constexpr bool F16 = std::is_same<T, _Float16>::value;
-  constexpr int QB = 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8, PT = win_pitch_tr(HK);
-  constexpr int STAGE = 2 * QB * PT + 2 * QB * 4;
-  constexpr int U = (QB * CH + 255) / 256;
+  constexpr int QB = HK <= 64 || HK > 128 ? 32 : 64;     // query rows of a tile: what three stages leave room for
+  constexpr int NQ = QB / 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8, PT = win_pitch_tr(HK);
+  constexpr int STAGE = 2 * QB * PT + 2 * QB * 4;        // Q | dO | lse2 | delta
+  constexpr int PX = NQ * 2048;                          // P of one key group: NQ x [2][64 lanes] x 16 bytes
+  constexpr int U = (QB * CH + 511) / 512;
   const WinArgs& p = a.w;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
-  __shared__ float sm_g[128];
+  __shared__ __attribute__((aligned(16))) unsigned char smem[3 * STAGE + 2 * 4 * PX];
+  __shared__ float sm_g[BW_KEYS];
   win_lds* const lds = (win_lds*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hi = lane >> 5, l31 = lane & 31;
+  const int hi = lane >> 5, l31 = lane & 31, kg = wave & 3;
+  const bool role = wave >> 2;
 
-  // block -> (batch entry, key head, key tile, query split); the longest tiles (sinks, then the first keys) come first
-  const int per = a.nst * a.sps + a.nrt * a.spr;
+  // block -> (key head, batch entry, key tile, query split); the longest tiles (sinks, then the first keys) come first
   int bid = blockIdx.x;
   const int hk = bid % p.kv_heads; bid /= p.kv_heads;
   const int b = bid % p.batch; bid /= p.batch;
   const bool sink = bid < a.nst * a.sps;
   const int loc = sink ? bid : bid - a.nst * a.sps, sp = sink ? a.sps : a.spr;
   const int tile = loc / sp, split = loc - tile * sp;
-  (void)per;
   const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk), shift = kn - qn;
   const int s_end = min(p.sinks, p.Lk);
   const int ka = (sink ? 0 : s_end) + tile * BW_KEYS, kz = min(ka + BW_KEYS, sink ? s_end : p.Lk), kb = min(kz, kn);
@@ -136,46 +143,48 @@ __global__ __launch_bounds__(256, HK <= 64 ? 2 : 1) void win_bwd_dkv_kernel(cons
   const int ntq = ib > ia ? (ib - ia + QB - 1) / QB : 0, its = ntq * p.group;
   const int itb = (int)((long)its * split / sp), ite = (int)((long)its * (split + 1) / sp);
 
-  const T* K = reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hk * p.k_hs;
-  const T* V = reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hk * p.v_hs;
-  const int kw = ka + wave * 32, key = kw + l31;
-  V8 kf[NKS], vf[NKS];
-  float vsq = 0.0f;
+  const T* W = role ? reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hk * p.v_hs
+                    : reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hk * p.k_hs;
+  const long w_rs = role ? p.v_rs : p.k_rs;
+  const int kw = ka + kg * 32, key = kw + l31;
+  V8 wf[NKS];                                    // this lane's key row of K (role 0) or V (role 1)
+  float wsq = 0.0f;
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) {
     const int d = ks * 16 + hi * 8;
-    const bool ok = key < kb && d < p.hd;
-    kf[ks] = ok ? ld8<T>(K + (long)key * p.k_rs + d) : zero8<T>();
-    vf[ks] = ok ? ld8<T>(V + (long)key * p.v_rs + d) : zero8<T>();
+    wf[ks] = key < kb && d < p.hd ? ld8<T>(W + (long)key * w_rs + d) : zero8<T>();
     if (F16)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { const float f = to_f32(vf[ks][e]); vsq += f * f; }
+      for (int e = 0; e < 8; ++e) { const float f = to_f32(wf[ks][e]); wsq += f * f; }
   }
   float gs = 1.0f;                               // fp16: scale of dS (relative to P's) for this lane's key
-  if (F16) {
+  if (F16 && role) {
     float dm = 0.0f;
     const float* m = a.domax + ((long)b * p.heads + hk * p.group) * a.nq64;
     for (int i = lane; i < p.group * a.nq64; i += 64) dm = fmaxf(dm, m[i]);
     dm = wave_max(dm);
-    const float g = ds_scale(dm, sqrtf(win_half_sum(vsq)));
-    if (hi == 0) sm_g[wave * 32 + l31] = 1.0f / g;
+    const float g = ds_scale(dm, sqrtf(win_half_sum(wsq)));
+    if (hi == 0) sm_g[kg * 32 + l31] = 1.0f / g;
     gs = g * 0x1p-14f;
   }
 
-  // positions that see this lane's key / that all of the wave's keys are seen from
-  const int plo = p.right < 0 ? -WIN_MAX_LEN * 2 + 1 : key - p.right, phi = p.left < 0 || sink ? WIN_MAX_LEN * 2 - 1 : key + p.left;
-  const int alo = p.right < 0 ? -WIN_MAX_LEN * 2 + 1 : kw + 31 - p.right, ahi = p.left < 0 || sink ? WIN_MAX_LEN * 2 - 1 : kw + p.left;
-  const int nlo = p.right < 0 ? -WIN_MAX_LEN * 2 + 1 : kw - p.right, nhi = p.left < 0 || sink ? WIN_MAX_LEN * 2 - 1 : kw + 31 + p.left;
+  // positions that see this lane's key / that all of the group's keys are seen from / that see any of them
+  constexpr int FAR = WIN_MAX_LEN * 2 - 1;
+  const bool back = p.left < 0 || sink;
+  const int plo = p.right < 0 ? -FAR : key - p.right, phi = back ? FAR : key + p.left;
+  const int alo = p.right < 0 ? -FAR : kw + 31 - p.right, ahi = back ? FAR : kw + p.left;
+  const int nlo = p.right < 0 ? -FAR : kw - p.right, nhi = back ? FAR : kw + 31 + p.left;
 
   V8 qr[U], gr[U];
   float lr = 0.0f, dr = 0.0f;
-  auto load = [&](int it) {
-    const int g = it / ntq, i0 = ia + (it - g * ntq) * QB, h = hk * p.group + g, rem = ib - i0;
+  int lg = ntq ? itb / ntq : 0, li = itb - lg * ntq;     // head of the group and query tile that load() takes next
+  auto load = [&]() {
+    const int i0 = ia + li * QB, h = hk * p.group + lg, rem = ib - i0;
     const T* qt = reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs + (long)i0 * p.q_rs;
     const T* gt = reinterpret_cast<const T*>(a.dout) + (long)b * a.do_bs + (long)h * a.do_hs + (long)i0 * a.do_rs;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+      const int u = tid + 512 * i, rr = u / CH, ch = u - rr * CH;
       const bool ok = rr < rem && rr < QB && ch * 8 < p.hd;
       qr[i] = ok ? ld8<T>(qt + (unsigned)rr * (unsigned)p.q_rs + ch * 8) : zero8<T>();
       gr[i] = ok ? ld8<T>(gt + (unsigned)rr * (unsigned)a.do_rs + ch * 8) : zero8<T>();
@@ -185,13 +194,14 @@ __global__ __launch_bounds__(256, HK <= 64 ? 2 : 1) void win_bwd_dkv_kernel(cons
       lr = tid < rem ? a.lse2[at] : __builtin_inff();
       dr = tid < rem ? a.delta[at] : 0.0f;
     }
+    if (++li == ntq) { li = 0; ++lg; }
   };
   auto store = [&](int stage) {
     win_lds* const qt = lds + stage * STAGE;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
-      if (QB * CH % 256 == 0 || u < QB * CH) {
+      const int u = tid + 512 * i, rr = u / CH, ch = u - rr * CH;
+      if (QB * CH % 512 == 0 || u < QB * CH) {
         *(__attribute__((address_space(3))) V8*)(qt + rr * PT + ch * 16) = qr[i];
         *(__attribute__((address_space(3))) V8*)(qt + QB * PT + rr * PT + ch * 16) = gr[i];
       }
@@ -202,83 +212,113 @@ __global__ __launch_bounds__(256, HK <= 64 ? 2 : 1) void win_bwd_dkv_kernel(cons
     }
   };
 
-  f32x16 dk[NDB], dv[NDB];
+  f32x16 acc[NDB];                               // dV (role 0) or dK (role 1): registers hold keys, lanes columns
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) dk[db][e] = dv[db][e] = 0.0f;
+    for (int e = 0; e < 16; ++e) acc[db][e] = 0.0f;
   const f32x16 zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  const int rfo = l31 * PT + hi * 16, tfo = (4 * hi + ((lane & 15) >> 2)) * PT + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+  // role 0 takes rows of Q and columns of dO, role 1 rows of dO and columns of Q
+  const int rfo = (role ? QB * PT : 0) + l31 * PT + hi * 16;
+  const int tfo = (role ? 0 : QB * PT) + (4 * hi + ((lane & 15) >> 2)) * PT + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+  win_lds* const px = lds + 3 * STAGE + kg * PX + lane * 16;
   const float c = p.c;
 
-  if (itb < ite) { load(itb); store(0); }
-  if (itb + 1 < ite) load(itb + 1);
+  if (itb < ite) { load(); store(0); }
+  if (itb + 1 < ite) load();
   __syncthreads();
-  for (int it = itb; it < ite; ++it) {
-    const int cur = (it - itb) & 1;
-    if (it + 1 < ite) store(cur ^ 1);
-    if (it + 2 < ite) load(it + 2);
-    const int p0 = shift + ia + (it % ntq) * QB;           // position of the tile's first row
-    const win_lds* const qt = lds + cur * STAGE;
-    const win_lds* const gt = qt + QB * PT;
-    const win_lds* const lt = qt + 2 * QB * PT;
-    if (kw < kb && p0 + QB - 1 >= nlo && p0 <= nhi) {
-      f32x16 s = zero16, dp = zero16;
+  int st = 0, ci = ntq ? itb % ntq : 0;          // stage and query tile of role 0; role 1 is one behind
+  int prev_p0 = 0;
+  for (int it = itb; it <= ite; ++it) {
+    const int nst = st == 2 ? 0 : st + 1, pst = st == 0 ? 2 : st - 1;
+    if (it + 1 < ite) store(nst);                // last read, by role 1, in the iteration before this one
+    if (it + 2 < ite) load();
+    const int p0 = role ? prev_p0 : shift + ia + ci * QB;
+    prev_p0 = shift + ia + ci * QB;
+    const bool mine = role ? it > itb : it < ite;
+    if (mine && kw < kb && p0 + QB - 1 >= nlo && p0 <= nhi) {
+      const win_lds* const tb = lds + (role ? pst : st) * STAGE;
+      const win_lds* const stat = tb + 2 * QB * PT + (role ? QB * 4 : 0) + 16 * hi;
+      win_lds* const pt = px + (((it - itb) ^ (role ? 1 : 0)) & 1) * 4 * PX;
+      f32x16 s[NQ];
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(qt + rfo + ks * 32), kf[ks], s);
+      for (int n = 0; n < NQ; ++n) {
+        s[n] = zero16;
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) dp = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(gt + rfo + ks * 32), vf[ks], dp);
-      const bool all = p0 >= alo && p0 + QB - 1 <= ahi;
-      V8 pf[2], df[2];
+        for (int ks = 0; ks < NKS; ++ks)
+          s[n] = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(tb + rfo + n * 32 * PT + ks * 32), wf[ks], s[n]);
+      }
+      V8 f[NQ][2];
+      if (!role) {
+        const bool all = p0 >= alo && p0 + QB - 1 <= ahi;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 ls = *(const __attribute__((address_space(3))) f32x4*)(lt + (8 * g + 4 * hi) * 4);
-        const f32x4 dl = *(const __attribute__((address_space(3))) f32x4*)(lt + QB * 4 + (8 * g + 4 * hi) * 4);
+        for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int x = 4 * g + e;
-          float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, (F16 ? P_EXP : 0.0f) - ls[e]));
-          if (!all) {
-            const int pe = p0 + 8 * g + 4 * hi + e;
-            pv = pe >= plo && pe <= phi ? pv : 0.0f;
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 ls = *(const __attribute__((address_space(3))) f32x4*)(stat + (n * 32 + 8 * g) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * g + e], c, (F16 ? P_EXP : 0.0f) - ls[e]));
           }
-          const float ds = F16 ? pv * ((dp[x] - dl[e]) * gs) : pv * (dp[x] - dl[e]);
-          pf[x >> 3][x & 7] = from_f32<T>(pv);
-          df[x >> 3][x & 7] = from_f32<T>(ds);
+          if (!all)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const int pe = p0 + n * 32 + 8 * (x >> 2) + 4 * hi + (x & 3);
+              s[n][x] = pe >= plo && pe <= phi ? s[n][x] : 0.0f;
+            }
+#pragma unroll
+          for (int x = 0; x < 16; ++x) f[n][x >> 3][x & 7] = from_f32<T>(s[n][x]);
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) *(__attribute__((address_space(3))) V8*)(pt + (n * 2 + h2) * 1024) = f[n][h2];
         }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) {
+            const V8 pv = *(const __attribute__((address_space(3))) V8*)(pt + (n * 2 + h2) * 1024);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const f32x4 dl = *(const __attribute__((address_space(3))) f32x4*)(stat + (n * 32 + 16 * h2 + 8 * g) * 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float dp = s[n][8 * h2 + 4 * g + e] - dl[e];
+                f[n][h2][4 * g + e] = from_f32<T>(to_f32(pv[4 * g + e]) * (F16 ? dp * gs : dp));
+              }
+            }
+          }
       }
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
         const int colb = min(db * 32 + gdh * 16, HK - 16) * 2;
 #pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2) {
-          dv[db] = Vec<T>::mfma32(pf[h2], win_tr8<V8, PT>(gt + tfo, h2 * 16, colb), dv[db]);
-          dk[db] = Vec<T>::mfma32(df[h2], win_tr8<V8, PT>(qt + tfo, h2 * 16, colb), dk[db]);
-        }
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) acc[db] = Vec<T>::mfma32(f[n][h2], win_tr8<V8, PT>(tb + tfo, n * 32 + h2 * 16, colb), acc[db]);
       }
     }
     __syncthreads();
+    st = nst;
+    if (++ci == ntq) ci = 0;
   }
-  // registers hold keys, lanes columns
   float* part = nullptr;
   if (sp > 1) {
     const int tp = sink ? loc : (a.sps > 1 ? a.nst * a.sps : 0) + loc;
-    part = a.part + (((long)b * p.kv_heads + hk) * a.nparts + tp) * BW_KEYS * 2 * p.hd;
+    part = a.part + (((long)b * p.kv_heads + hk) * a.nparts + tp) * BW_KEYS * 2 * p.hd + (role ? 0 : p.hd);
   }
-  T* dK = reinterpret_cast<T*>(a.dk) + (long)b * a.dk_bs + (long)hk * a.dk_hs;
-  T* dV = reinterpret_cast<T*>(a.dv) + (long)b * a.dv_bs + (long)hk * a.dv_hs;
+  T* D = role ? reinterpret_cast<T*>(a.dk) + (long)b * a.dk_bs + (long)hk * a.dk_hs
+              : reinterpret_cast<T*>(a.dv) + (long)b * a.dv_bs + (long)hk * a.dv_hs;
+  const long d_rs = role ? a.dk_rs : a.dv_rs;
 #pragma unroll
   for (int db = 0; db < NDB; ++db) {
     const int d = db * 32 + l31;
     if (d >= p.hd) continue;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int kl = wave * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi, j = ka + kl;
-      const bool live = j < kb;
-      const float gk = live ? dk[db][e] * (F16 ? sm_g[kl] * p.scale : p.scale) : 0.0f;
-      const float gv = live ? (F16 ? dv[db][e] * 0x1p-14f : dv[db][e]) : 0.0f;
-      if (part) { part[(long)kl * 2 * p.hd + d] = gk; part[(long)kl * 2 * p.hd + p.hd + d] = gv; }
-      else if (j < kz) { dK[(long)j * a.dk_rs + d] = from_f32<T>(gk); dV[(long)j * a.dv_rs + d] = from_f32<T>(gv); }
+      const int kl = kg * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi, j = ka + kl;
+      const float f = role ? (F16 ? sm_g[kl] * p.scale : p.scale) : (F16 ? 0x1p-14f : 1.0f);
+      const float v = j < kb ? acc[db][e] * f : 0.0f;
+      if (part) part[(long)kl * 2 * p.hd + d] = v;
+      else if (j < kz) D[(long)j * d_rs + d] = from_f32<T>(v);
     }
   }
 }
@@ -312,7 +352,7 @@ __global__ __launch_bounds__(256) void win_bwd_join_kernel(const WinBwdArgs a) {
 }
 
 template <typename T, int HK>
-__global__ __launch_bounds__(256, HK <= 64 ? 2 : 1) void win_bwd_dq_kernel(const WinBwdArgs a) {
+__global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) {
   using V8 = typename Vec<T>::v8;
   using V4 = typename Vec<T>::v4;
   constexpr bool F16 = std::is_same<T, _Float16>::value;
@@ -494,7 +534,7 @@ int launch_hk(const WinBwdArgs& a, hipStream_t st) {
   const WinArgs& p = a.w;
   const long tiles = (long)p.batch * p.kv_heads * (a.nst * a.sps + a.nrt * a.spr);
   if (tiles > 0) {
-    hipLaunchKernelGGL((win_bwd_dkv_kernel<T, HK>), dim3((unsigned)tiles), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((win_bwd_dkv_kernel<T, HK>), dim3((unsigned)tiles), dim3(512), 0, st, a);
     HALLO_CHECK_LAUNCH();
   }
   if (p.Lq > 0) {
