@@ -38,22 +38,44 @@ __device__ __forceinline__ WinRange win_range(const WinArgs& p, int plo, int phi
   return lo <= se ? WinRange{hi, hi, hi} : WinRange{se, lo, hi};
 }
 
-// LDS row pitches in bytes for rows of HK elements (a multiple of 16).  Rows that are only read as MFMA fragments along the row (16
-// bytes per lane, lane = row): an odd number of 16-byte slots, so consecutive rows start on different banks.  Rows that are read
-// transposed (4 rows x 32 bytes per 16 lanes): twice an odd number, so that those four pieces are on different banks.
-constexpr int win_pitch_row(int HK) { return HK * 2 + 16; }
-constexpr int win_pitch_tr(int HK) { return HK * 2 + ((HK / 16) % 2 ? 0 : 32); }
-
-// Operand of a 32x32x16 MFMA whose 16-deep contraction runs over 16 LDS rows, read transposed: lane l holds column
-// col0 + (l & 31) of rows row0 + 4 hi + (e & 3) + 8 (e >> 2) (hi = l >> 5, e = 0..7) -- the rows in which a 32x32 accumulator of the
-// same wave holds its registers, so a converted accumulator is the other operand as it stands.
-// `base`: tile + ((l >> 5) * 4 + ((l & 15) >> 2)) * pitch + (l & 3) * 8 ; colb: byte offset of this lane's 16-column group
-template <typename V8, int PITCH>
-__device__ __forceinline__ V8 win_tr8(const win_lds* base, int row0, int colb) {
-  const win_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) win_s16x4*)(base + row0 * PITCH + colb));
-  const win_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) win_s16x4*)(base + (row0 + 8) * PITCH + colb));
-  return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+// LDS tiles of rows of HK elements (a multiple of 16): rows of win_chunks(HK) 16-byte chunks, chunk c of row r stored at c ^ win_swz(r).
+// A tile is read along its rows (MFMA operand, 16 bytes per lane, lane = row: 16 consecutive rows at one chunk) and transposed (32
+// lanes: 4 consecutive rows x 64 aligned bytes); the swizzle puts both kinds of 256 bytes on all 64 banks once.  It repeats every 16
+// rows, so a fragment further down the tile is an immediate offset away.  (Padded pitches without a swizzle serve one kind only: a
+// quarter of the forward kernel's LDS cycles were conflicts.)
+constexpr int win_chunks(int HK) { return HK == 48 ? 8 : HK == 80 ? 12 : HK == 112 ? 16 : HK == 144 ? 20 : HK / 8; }
+template <int HK> __device__ __forceinline__ int win_swz(int r) {
+  constexpr int C = win_chunks(HK);
+  return C == 16 ? (r & 3) << 2 | (r >> 2 & 3) : C == 8 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : C == 2 ? r >> 3 & 1 : r >> 2 & 3;
 }
+template <int HK> struct WinTile {
+  static constexpr int CH = HK / 8, PITCH = win_chunks(HK) * 16, NKS = HK / 16, NDB = (HK + 31) / 32;
+  static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ win_swz<HK>(r)) << 4); }
+  // this lane's byte offsets: along[ks] of row (lane & 31), columns 16 ks + 8 hi; trans[db][k] of rows 8 k + .. read transposed
+  int along[NKS], trans[NDB][2];
+  __device__ __forceinline__ WinTile(int lane) {
+    const int hi = lane >> 5, l31 = lane & 31, gi = lane & 15, gdh = lane >> 4 & 1;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) along[ks] = at(l31, ks * 2 + hi);
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)                // columns past HK: operand rows whose products are not stored
+        trans[db][k] = at(8 * k + 4 * hi + (gi >> 2), min(db * 4 + gdh * 2, CH - 2) + (gi >> 1 & 1)) + (gi & 1) * 8;
+  }
+  template <typename V8> __device__ __forceinline__ V8 row(const win_lds* tile, int row0, int ks) const {
+    return *(const __attribute__((address_space(3))) V8*)(tile + along[ks] + row0 * PITCH);
+  }
+  // Operand of a 32x32x16 MFMA whose 16-deep contraction runs over 16 LDS rows, read transposed: lane l holds column db * 32 + (l & 31)
+  // of rows row0 + 4 hi + (e & 3) + 8 (e >> 2) (e = 0..7) -- the rows in which a 32x32 accumulator of the same wave holds its
+  // registers, so a converted accumulator is the other operand as it stands.  row0: a multiple of 16
+  template <typename V8> __device__ __forceinline__ V8 col(const win_lds* tile, int row0, int db) const {
+    typedef __attribute__((address_space(3))) win_s16x4 lds4;
+    const win_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + trans[db][0] + row0 * PITCH));
+    const win_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + trans[db][1] + row0 * PITCH));
+    return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
 
 // maximum / sum with the partner lane (l ^ 32).  The swap is written out: s_nop 1 covers the VALU write -> permlane read hazard, and
 // through the builtin hipcc folds max(a, b) of the swapped pair to a.

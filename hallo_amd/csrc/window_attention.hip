@@ -24,7 +24,8 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
   using V4 = typename Vec<T>::v4;
   constexpr int KB = HK > 128 ? 32 : 64;         // keys per tile
   constexpr int NT = KB / 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8;
-  constexpr int KP = win_pitch_row(HK), VP = win_pitch_tr(HK), STAGE = KB * (KP + VP);
+  using Tile = WinTile<HK>;
+  constexpr int TB = KB * Tile::PITCH, STAGE = 2 * TB;   // K | V
   constexpr int U = (KB * CH + 255) / 256;       // 16-byte pieces per thread and tensor
   constexpr float NEG_INF = -__builtin_inff();
   __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
@@ -83,8 +84,8 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
     for (int i = 0; i < U; ++i) {
       const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
       if (KB * CH % 256 == 0 || u < KB * CH) {
-        *(__attribute__((address_space(3))) V8*)(kt + rr * KP + ch * 16) = kr[i];
-        *(__attribute__((address_space(3))) V8*)(kt + KB * KP + rr * VP + ch * 16) = vr[i];
+        *(__attribute__((address_space(3))) V8*)(kt + Tile::at(rr, ch)) = kr[i];
+        *(__attribute__((address_space(3))) V8*)(kt + TB + Tile::at(rr, ch)) = vr[i];
       }
     }
   };
@@ -97,8 +98,7 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
   float m = NEG_INF, l = 0.0f;
   const float c = p.c, slack = 6.0f / p.c;
   const f32x16 zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  const int kfo = l31 * KP + hi * 16;
-  const int vfo = (4 * hi + ((lane & 15) >> 2)) * VP + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+  const Tile tl(lane);
 
   if (nt > 0) { load(0); store(0); }
   if (nt > 1) load(1);
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
     if (t + 1 < nt) store((t + 1) & 1);          // read last in iteration t - 1, which the barrier below closed
     if (t + 2 < nt) load(t + 2);
     const win_lds* const kt = lds + (t & 1) * STAGE;
-    const win_lds* const vt = kt + KB * KP;
+    const win_lds* const vt = kt + TB;
     const bool none = iw >= qn || (p.right >= 0 && j0 > pw1 + p.right) || (p.left >= 0 && j0 + KB <= pw0 - p.left && j0 >= p.sinks);
     if (!none) {
       f32x16 s[NT];
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
         s[n] = zero16;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
-          s[n] = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(kt + kfo + n * 32 * KP + ks * 32), qf[ks], s[n]);
+          s[n] = Vec<T>::mfma32(tl.template row<V8>(kt, n * 32, ks), qf[ks], s[n]);
       }
       const bool all = end - j0 >= KB && (p.right < 0 || j0 + KB - 1 <= pw0 + p.right) &&
                        (p.left < 0 || j0 >= pw1 - p.left || j0 + KB <= p.sinks);
@@ -131,12 +131,12 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
             s[n][e] = j < lhi && (j >= vlo || j < p.sinks) ? s[n][e] : NEG_INF;
           }
       }
-      float mt = NEG_INF;
+      float mx[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};    // four chains: a dependent chain of 32 would be latency
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[n][e]);
-      mt = win_half_max(mt);
+        for (int e = 0; e < 16; e += 2) mx[e / 2 & 3] = fmaxf(fmaxf(s[n][e], s[n][e + 1]), mx[e / 2 & 3]);
+      const float mt = win_half_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
       if (__any(mt > m + slack)) {
         const float mn = fmaxf(m, mt);
         const float a = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);     // m = -inf: 0
@@ -149,23 +149,23 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
       }
       const float mc = m == NEG_INF ? 0.0f : m * c;
       V8 pf[NT][2];
+      float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], c, -mc));
-          l += pv;
+          ls[e & 3] += pv;
           pf[n][e >> 3][e & 7] = from_f32<T>(pv);
         }
+      l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const int colb = min(db * 32 + gdh * 16, HK - 16) * 2;     // columns past HK: rows of O^T that are not stored
+      for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int h2 = 0; h2 < 2; ++h2)
-            o[db] = Vec<T>::mfma32(win_tr8<V8, VP>(vt + vfo, n * 32 + h2 * 16, colb), pf[n][h2], o[db]);
-      }
+            o[db] = Vec<T>::mfma32(tl.template col<V8>(vt, n * 32 + h2 * 16, db), pf[n][h2], o[db]);
     }
     __syncthreads();
   }
@@ -200,9 +200,10 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
 template <typename T, int HK>
 __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   using V8 = typename Vec<T>::v8;
-  constexpr int NKS = HK / 16, NDB = (HK + 31) / 32, VP = win_pitch_tr(HK), OP = HK + 4;      // OP: pitch of the joined rows, floats
+  constexpr int NKS = HK / 16, NDB = (HK + 31) / 32, OP = HK + 4;      // OP: pitch of the joined rows, floats
   constexpr float NEG_INF = -__builtin_inff();
-  constexpr int VT = 4 * 32 * VP, JT = 32 * OP * 4;
+  using Tile = WinTile<HK>;
+  constexpr int VT = 4 * 32 * Tile::PITCH, JT = 32 * OP * 4;
   __shared__ __attribute__((aligned(16))) unsigned char smem[VT > JT ? VT : JT];
   __shared__ float sm_m[4][32], sm_l[4][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -253,8 +254,8 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
     for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
   float m = NEG_INF, l = 0.0f;
   const float c = p.c;
-  win_lds* const vt = (win_lds*)smem + wave * 32 * VP;
-  const int vfo = (4 * hi + ((lane & 15) >> 2)) * VP + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+  win_lds* const vt = (win_lds*)smem + wave * 32 * Tile::PITCH;
+  const Tile tl(lane);
 
   int t = tb + wave;
   if (t < te) load(t);
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(kr[ks], qf[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) *(__attribute__((address_space(3))) V8*)(vt + l31 * VP + (ks * 16 + hi * 8) * 2) = vr[ks];
+    for (int ks = 0; ks < NKS; ++ks) *(__attribute__((address_space(3))) V8*)(vt + tl.along[ks]) = vr[ks];
     const int j0 = t < n0 ? t * 32 : w.s1 + (t - n0) * 32, end = t < n0 ? w.e0 : w.e1;
     if (t + 4 < te) load(t + 4);
     const bool all = end - j0 >= 32 && (p.right < 0 || j0 + 31 <= plo + p.right) && (p.left < 0 || j0 >= phi - p.left || j0 + 32 <= p.sinks);
@@ -298,11 +299,9 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
       pf[e >> 3][e & 7] = from_f32<T>(pv);
     }
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) {
-      const int colb = min(db * 32 + gdh * 16, HK - 16) * 2;
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) o[db] = Vec<T>::mfma32(win_tr8<V8, VP>(vt + vfo, h2 * 16, colb), pf[h2], o[db]);
-    }
+      for (int h2 = 0; h2 < 2; ++h2) o[db] = Vec<T>::mfma32(tl.template col<V8>(vt, h2 * 16, db), pf[h2], o[db]);
   }
   l = win_half_sum(l);
   if (!live) { m = NEG_INF; l = 0.0f; }          // rows without a query went along in the tiles that need no mask

@@ -111,8 +111,9 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
   using V8 = typename Vec<T>::v8;
   constexpr bool F16 = std::is_same<T, _Float16>::value;
   constexpr int QB = HK <= 64 || HK > 128 ? 32 : 64;     // query rows of a tile: what three stages leave room for
-  constexpr int NQ = QB / 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8, PT = win_pitch_tr(HK);
-  constexpr int STAGE = 2 * QB * PT + 2 * QB * 4;        // Q | dO | lse2 | delta
+  constexpr int NQ = QB / 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8;
+  using Tile = WinTile<HK>;
+  constexpr int TB = QB * Tile::PITCH, STAGE = 2 * TB + 2 * QB * 4;        // Q | dO | lse2 | delta
   constexpr int PX = NQ * 2048;                          // P of one key group: NQ x [2][64 lanes] x 16 bytes
   constexpr int U = (QB * CH + 511) / 512;
   const WinArgs& p = a.w;
@@ -202,13 +203,13 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
     for (int i = 0; i < U; ++i) {
       const int u = tid + 512 * i, rr = u / CH, ch = u - rr * CH;
       if (QB * CH % 512 == 0 || u < QB * CH) {
-        *(__attribute__((address_space(3))) V8*)(qt + rr * PT + ch * 16) = qr[i];
-        *(__attribute__((address_space(3))) V8*)(qt + QB * PT + rr * PT + ch * 16) = gr[i];
+        *(__attribute__((address_space(3))) V8*)(qt + Tile::at(rr, ch)) = qr[i];
+        *(__attribute__((address_space(3))) V8*)(qt + TB + Tile::at(rr, ch)) = gr[i];
       }
     }
     if (tid < QB) {
-      *(__attribute__((address_space(3))) float*)(qt + 2 * QB * PT + tid * 4) = lr;
-      *(__attribute__((address_space(3))) float*)(qt + 2 * QB * PT + QB * 4 + tid * 4) = dr;
+      *(__attribute__((address_space(3))) float*)(qt + 2 * TB + tid * 4) = lr;
+      *(__attribute__((address_space(3))) float*)(qt + 2 * TB + QB * 4 + tid * 4) = dr;
     }
   };
 
@@ -219,8 +220,8 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
     for (int e = 0; e < 16; ++e) acc[db][e] = 0.0f;
   const f32x16 zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
   // role 0 takes rows of Q and columns of dO, role 1 rows of dO and columns of Q
-  const int rfo = (role ? QB * PT : 0) + l31 * PT + hi * 16;
-  const int tfo = (role ? 0 : QB * PT) + (4 * hi + ((lane & 15) >> 2)) * PT + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+  const int rfo = role ? TB : 0, tfo = role ? 0 : TB;
+  const Tile tl(lane);
   win_lds* const px = lds + 3 * STAGE + kg * PX + lane * 16;
   const float c = p.c;
 
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
     const bool mine = role ? it > itb : it < ite;
     if (mine && kw < kb && p0 + QB - 1 >= nlo && p0 <= nhi) {
       const win_lds* const tb = lds + (role ? pst : st) * STAGE;
-      const win_lds* const stat = tb + 2 * QB * PT + (role ? QB * 4 : 0) + 16 * hi;
+      const win_lds* const stat = tb + 2 * TB + (role ? QB * 4 : 0) + 16 * hi;
       win_lds* const pt = px + (((it - itb) ^ (role ? 1 : 0)) & 1) * 4 * PX;
       f32x16 s[NQ];
 #pragma unroll
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
         s[n] = zero16;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
-          s[n] = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(tb + rfo + n * 32 * PT + ks * 32), wf[ks], s[n]);
+          s[n] = Vec<T>::mfma32(tl.template row<V8>(tb + rfo, n * 32, ks), wf[ks], s[n]);
       }
       V8 f[NQ][2];
       if (!role) {
@@ -288,13 +289,11 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
           }
       }
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const int colb = min(db * 32 + gdh * 16, HK - 16) * 2;
+      for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2) acc[db] = Vec<T>::mfma32(f[n][h2], win_tr8<V8, PT>(tb + tfo, n * 32 + h2 * 16, colb), acc[db]);
-      }
+          for (int h2 = 0; h2 < 2; ++h2) acc[db] = Vec<T>::mfma32(f[n][h2], tl.template col<V8>(tb + tfo, n * 32 + h2 * 16, db), acc[db]);
     }
     __syncthreads();
     st = nst;
@@ -357,7 +356,8 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
   using V4 = typename Vec<T>::v4;
   constexpr bool F16 = std::is_same<T, _Float16>::value;
   constexpr int KB = 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8;
-  constexpr int PT = win_pitch_tr(HK), VP = win_pitch_row(HK), STAGE = KB * (PT + VP);
+  using Tile = WinTile<HK>;
+  constexpr int TB = KB * Tile::PITCH, STAGE = 2 * TB;   // K | V
   constexpr int U = (KB * CH + 255) / 256;
   const WinArgs& p = a.w;
   __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
@@ -426,8 +426,8 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
     for (int i = 0; i < U; ++i) {
       const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
       if (KB * CH % 256 == 0 || u < KB * CH) {
-        *(__attribute__((address_space(3))) V8*)(kt + rr * PT + ch * 16) = kr[i];
-        *(__attribute__((address_space(3))) V8*)(kt + KB * PT + rr * VP + ch * 16) = vr[i];
+        *(__attribute__((address_space(3))) V8*)(kt + Tile::at(rr, ch)) = kr[i];
+        *(__attribute__((address_space(3))) V8*)(kt + TB + Tile::at(rr, ch)) = vr[i];
       }
     }
   };
@@ -437,8 +437,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
 #pragma unroll
     for (int e = 0; e < 16; ++e) dq[db][e] = 0.0f;
   const f32x16 zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  const int kfo = l31 * PT + hi * 16, vfo = l31 * VP + hi * 16;
-  const int tfo = (4 * hi + ((lane & 15) >> 2)) * PT + (lane & 3) * 8, gdh = (lane >> 4) & 1;
+  const Tile tl(lane);
   const float c = p.c;
 
   if (nt > 0) { load(0); store(0); }
@@ -449,14 +448,14 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
     if (t + 1 < nt) store((t + 1) & 1);
     if (t + 2 < nt) load(t + 2);
     const win_lds* const kt = lds + (t & 1) * STAGE;
-    const win_lds* const vt = kt + KB * PT;
+    const win_lds* const vt = kt + TB;
     const bool none = iw >= qn || (p.right >= 0 && j0 > pw1 + p.right) || (p.left >= 0 && j0 + KB <= pw0 - p.left && j0 >= p.sinks);
     if (!none) {
       f32x16 s = zero16, dp = zero16;
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(kt + kfo + ks * 32), qf[ks], s);
+      for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(tl.template row<V8>(kt, 0, ks), qf[ks], s);
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) dp = Vec<T>::mfma32(*(const __attribute__((address_space(3))) V8*)(vt + vfo + ks * 32), gf[ks], dp);
+      for (int ks = 0; ks < NKS; ++ks) dp = Vec<T>::mfma32(tl.template row<V8>(vt, 0, ks), gf[ks], dp);
       const bool all = end - j0 >= KB && (p.right < 0 || j0 + KB - 1 <= pw0 + p.right) &&
                        (p.left < 0 || j0 >= pw1 - p.left || j0 + KB <= p.sinks);
       const int lhi = min(vhi, end);
@@ -471,11 +470,9 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
         df[e >> 3][e & 7] = from_f32<T>(pv * (dp[e] - delta));
       }
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const int colb = min(db * 32 + gdh * 16, HK - 16) * 2;
+      for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2) dq[db] = Vec<T>::mfma32(win_tr8<V8, PT>(kt + tfo, h2 * 16, colb), df[h2], dq[db]);
-      }
+        for (int h2 = 0; h2 < 2; ++h2) dq[db] = Vec<T>::mfma32(tl.template col<V8>(kt, h2 * 16, db), df[h2], dq[db]);
     }
     __syncthreads();
   }
