@@ -77,6 +77,23 @@ template <int HK> struct WinTile {
   }
 };
 
+// Order of a stretch of code that holds `mfmas` MFMAs with `per` LDS reads each and nothing else of either kind: `ahead` MFMAs' reads
+// first, then an MFMA and the reads of the one `ahead` places later, in turn.  (hipcc's own order puts each read right in front of its
+// MFMA, so that every MFMA waits for a read's whole latency.)
+template <int mfmas, int per, int ahead> __device__ __forceinline__ void win_order() {
+  __builtin_amdgcn_sched_group_barrier(0x100, per * ahead, 0);
+#pragma unroll
+  for (int i = 0; i < mfmas - ahead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, per, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, ahead, 0);
+}
+
+// Wait for all loads issued so far (vmcnt 0).  Put behind the loads that stay in registers for a whole loop: hipcc cannot see that they
+// have arrived once loads of the loop's own are in flight on the way round, and would wait for those in every iteration.
+__device__ __forceinline__ void win_loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // maximum / sum with the partner lane (l ^ 32).  The swap is written out: s_nop 1 covers the VALU write -> permlane read hazard, and
 // through the builtin hipcc folds max(a, b) of the swapped pair to a.
 __device__ __forceinline__ float win_half_max(float v) {

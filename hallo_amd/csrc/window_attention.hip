@@ -19,7 +19,7 @@ namespace hallo {
 namespace {
 
 template <typename T, int HK>
-__global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const WinArgs p) {
+__global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
   using V8 = typename Vec<T>::v8;
   using V4 = typename Vec<T>::v4;
   constexpr int KB = HK > 128 ? 32 : 64;         // keys per tile
@@ -33,10 +33,13 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, l31 = lane & 31;
-  int bid = xcd_remap(blockIdx.x, p.batch * p.heads * p.nqb);      // the blocks of a key head stay in one XCD's L2
+  // the blocks of a key head stay in one XCD's L2, the heads that share it side by side
+  int bid = xcd_remap(blockIdx.x, p.batch * p.heads * p.nqb);
+  const int gh = bid % p.group;
+  bid /= p.group;
   const int qb = p.nqb - 1 - bid % p.nqb;        // causal masks: the blocks with the most keys first
   bid /= p.nqb;
-  const int h = bid % p.heads, b = bid / p.heads, hk = h / p.group;
+  const int hk = bid % p.kv_heads, b = bid / p.kv_heads, h = hk * p.group + gh;
   const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk);
   const T* Q = reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs;
   const T* K = reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hk * p.k_hs;
@@ -101,6 +104,7 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
   const Tile tl(lane);
 
   if (nt > 0) { load(0); store(0); }
+  win_loads_done();
   if (nt > 1) load(1);
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
@@ -119,6 +123,7 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
         for (int ks = 0; ks < NKS; ++ks)
           s[n] = Vec<T>::mfma32(tl.template row<V8>(kt, n * 32, ks), qf[ks], s[n]);
       }
+      win_order<NT * NKS, 1, NKS < 4 ? NKS : 4>();
       const bool all = end - j0 >= KB && (p.right < 0 || j0 + KB - 1 <= pw0 + p.right) &&
                        (p.left < 0 || j0 >= pw1 - p.left || j0 + KB <= p.sinks);
       if (!all) {
@@ -166,6 +171,7 @@ __global__ __launch_bounds__(256, HK <= 128 ? 2 : 1) void win_fwd_kernel(const W
 #pragma unroll
           for (int h2 = 0; h2 < 2; ++h2)
             o[db] = Vec<T>::mfma32(tl.template col<V8>(vt, n * 32 + h2 * 16, db), pf[n][h2], o[db]);
+      win_order<NDB * NT * 2, 2, NDB * NT * 2 < 4 ? 2 : 4>();
     }
     __syncthreads();
   }

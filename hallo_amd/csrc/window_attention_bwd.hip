@@ -226,6 +226,7 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
   const float c = p.c;
 
   if (itb < ite) { load(); store(0); }
+  win_loads_done();
   if (itb + 1 < ite) load();
   __syncthreads();
   int st = 0, ci = ntq ? itb % ntq : 0;          // stage and query tile of role 0; role 1 is one behind
@@ -249,6 +250,7 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
         for (int ks = 0; ks < NKS; ++ks)
           s[n] = Vec<T>::mfma32(tl.template row<V8>(tb + rfo, n * 32, ks), wf[ks], s[n]);
       }
+      win_order<NQ * NKS, 1, NKS < 4 ? NKS : 4>();
       V8 f[NQ][2];
       if (!role) {
         const bool all = p0 >= alo && p0 + QB - 1 <= ahi;
@@ -294,6 +296,7 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
           for (int h2 = 0; h2 < 2; ++h2) acc[db] = Vec<T>::mfma32(f[n][h2], tl.template col<V8>(tb + tfo, n * 32 + h2 * 16, db), acc[db]);
+      win_order<NDB * NQ * 2, 2, NDB * NQ * 2 < 4 ? 2 : 4>();
     }
     __syncthreads();
     st = nst;
@@ -441,6 +444,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
   const float c = p.c;
 
   if (nt > 0) { load(0); store(0); }
+  win_loads_done();
   if (nt > 1) load(1);
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
@@ -456,6 +460,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
       for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(tl.template row<V8>(kt, 0, ks), qf[ks], s);
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) dp = Vec<T>::mfma32(tl.template row<V8>(vt, 0, ks), gf[ks], dp);
+      win_order<2 * NKS, 1, NKS < 4 ? NKS : 4>();
       const bool all = end - j0 >= KB && (p.right < 0 || j0 + KB - 1 <= pw0 + p.right) &&
                        (p.left < 0 || j0 >= pw1 - p.left || j0 + KB <= p.sinks);
       const int lhi = min(vhi, end);
@@ -473,6 +478,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int h2 = 0; h2 < 2; ++h2) dq[db] = Vec<T>::mfma32(tl.template col<V8>(kt, h2 * 16, db), df[h2], dq[db]);
+      win_order<NDB * 2, 2, NDB * 2 < 4 ? 2 : 4>();
     }
     __syncthreads();
   }
