@@ -6,7 +6,7 @@
 //
 // Both directions are bound by HBM: x (and dy) is read once, the result written once, everything between lives in registers.  A
 // row of nvec = ceil(C / 8) 16-byte vectors is shared by LPR lanes with VPL vectors each, so that a narrow row does not idle lanes
-// (C = 320: 8 lanes x 5 vectors, 8 rows per wave) and a wide one stays in registers (LPR = 256: the whole workgroup on a row).
+// (C = 320: 16 lanes x 3 vectors, 4 rows per wave) and a wide one stays in registers (LPR = 256: the whole workgroup on a row).
 // The row sums go through a fixed tree of lane exchanges, the weight gradients through a fixed sequence -- lane, lanes of a wave,
 // waves of a workgroup, workgroups in the second launch -- so a result does not depend on timing (no atomics).
 #include "common.h"
@@ -16,19 +16,19 @@ namespace hallo {
 
 namespace {
 
-// 8 elements at 2-byte alignment (rows of odd length or odd pitch): gfx950 global loads take any alignment
-template <typename T> struct __attribute__((packed, aligned(2))) U8 { typename Vec<T>::v8 v; };
+// 8 elements at their own alignment (rows of odd length or odd pitch): gfx950 global loads and stores take any
+template <typename V, int A> struct __attribute__((packed, aligned(A))) Loose { V v; };
 
+// columns col .. col + 7 of a row of C as they are stored, zeros past its end
 template <typename T, bool AL>
-__device__ __forceinline__ void ld_row8(const T* p, int col, int C, float (&f)[8]) {
-  if (AL || col + 8 <= C) {
-    const typename Vec<T>::v8 t = AL ? ld8<T>(p + col) : reinterpret_cast<const U8<T>*>(p + col)->v;
+__device__ __forceinline__ typename Vec<T>::v8 ld_raw8(const T* p, int col, int C) {
+  if (AL) return ld8<T>(p + col);
+  if (col + 8 <= C) return reinterpret_cast<const Loose<typename Vec<T>::v8, 2>*>(p + col)->v;
+  typename Vec<T>::v8 t = zero8<T>();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = to_f32(t[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = col + e < C ? to_f32(p[col + e]) : 0.0f;
-  }
+  for (int e = 0; e < 8; ++e)
+    if (col + e < C) t[e] = p[col + e];
+  return t;
 }
 template <typename T, bool AL>
 __device__ __forceinline__ void st_row8(T* p, int col, int C, const float (&f)[8]) {
@@ -36,7 +36,7 @@ __device__ __forceinline__ void st_row8(T* p, int col, int C, const float (&f)[8
 #pragma unroll
   for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(f[e]);
   if (AL) st8<T>(p + col, t);
-  else if (col + 8 <= C) reinterpret_cast<U8<T>*>(p + col)->v = t;
+  else if (col + 8 <= C) reinterpret_cast<Loose<typename Vec<T>::v8, 2>*>(p + col)->v = t;
   else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -46,10 +46,24 @@ __device__ __forceinline__ void st_row8(T* p, int col, int C, const float (&f)[8
 // weights: the activations' type or fp32 (master weights), absent = `dflt`
 template <typename T>
 __device__ __forceinline__ void ld_weight8(const void* w, int f32, int col, int C, float dflt, float (&f)[8]) {
+  if (!w) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int c = min(col + e, C - 1);
-    f[e] = !w ? dflt : (f32 ? reinterpret_cast<const float*>(w)[c] : to_f32(reinterpret_cast<const T*>(w)[c]));
+    for (int e = 0; e < 8; ++e) f[e] = dflt;
+  } else if (col + 8 > C) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = min(col + e, C - 1);
+      f[e] = f32 ? reinterpret_cast<const float*>(w)[c] : to_f32(reinterpret_cast<const T*>(w)[c]);
+    }
+  } else if (f32) {
+    typedef __attribute__((ext_vector_type(8))) float f32x8;
+    const f32x8 t = reinterpret_cast<const Loose<f32x8, 4>*>(reinterpret_cast<const float*>(w) + col)->v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = t[e];
+  } else {
+    const typename Vec<T>::v8 t = reinterpret_cast<const Loose<typename Vec<T>::v8, 2>*>(reinterpret_cast<const T*>(w) + col)->v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = to_f32(t[e]);
   }
 }
 
@@ -77,20 +91,18 @@ __global__ __launch_bounds__(256) void ln_train_kernel(const T* x, long ldx, T* 
   const bool live = row < rows;                  // LPR = 256: one row per workgroup, always live
   const T* xr = x + (live ? row : 0) * ldx;
   const int nvec = (C + 7) / 8;
+  typename Vec<T>::v8 raw[VPL];
   float v[VPL][8];
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     const int vi = sub + LPR * i;
-    if (vi < nvec) ld_row8<T, AL>(xr, vi * 8, C, v[i]);
-    else
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+    raw[i] = vi < nvec ? ld_raw8<T, AL>(xr, vi * 8, C) : zero8<T>();
   }
 #pragma unroll
   for (int i = 0; i < VPL; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum += v[i][e];
+    for (int e = 0; e < 8; ++e) { v[i][e] = to_f32(raw[i][e]); sum += v[i][e]; }
   const float mean = row_sum<LPR>(sum, red, 0) / (float)C;
   float sq = 0.0f;
 #pragma unroll
@@ -137,46 +149,59 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* dy, long ldd, cons
 #pragma unroll
     for (int e = 0; e < 8; ++e) ag[i][e] = ab[i][e] = 0.0f;
   }
-  int slot = 0;
-  for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += (long)gridDim.x * RPB) {
-    const long row = r0 + threadIdx.x / LPR;
+  // The row group after next is requested before a group is worked on: raw 16-byte vectors wait in registers, and are converted once
+  // for the sums and once more for dx (fp32 copies of both inputs would cost the second wave of a SIMD).
+  using V8 = typename Vec<T>::v8;
+  V8 xr[VPL], dr[VPL];
+  float2 st;
+  const long step = (long)gridDim.x * RPB;
+  auto load = [&](long row) {
     const bool live = row < rows;                // dead lanes (last group) carry zeros through the sums
-    const long rr = live ? row : 0;
-    const float2 st = stats[rr];
-    float xh[VPL][8], d[VPL][8];
+    st = stats[live ? row : 0];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int vi = sub + LPR * i;
-      if (live && vi < nvec) {
-        ld_row8<T, AL>(x + rr * ldx, vi * 8, C, xh[i]);
-        ld_row8<T, AL>(dy + rr * ldd, vi * 8, C, d[i]);
-      } else
-#pragma unroll
-        for (int e = 0; e < 8; ++e) xh[i][e] = d[i][e] = 0.0f;
+      xr[i] = live && vi < nvec ? ld_raw8<T, AL>(x + row * ldx, vi * 8, C) : zero8<T>();
+      dr[i] = live && vi < nvec ? ld_raw8<T, AL>(dy + row * ldd, vi * 8, C) : zero8<T>();
     }
+  };
+  int slot = 0;
+  long row = (long)blockIdx.x * RPB + threadIdx.x / LPR;
+  load(row);
+  for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += step, row += step) {
+    V8 xc[VPL], dc[VPL];
+    const float mean = st.x, rstd = st.y;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) { xc[i] = xr[i]; dc[i] = dr[i]; }
+    if (r0 + step < rows) load(row + step);
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        xh[i][e] = (xh[i][e] - st.x) * st.y;     // columns past C and dead rows meet d = 0
-        if (WG) { ag[i][e] += d[i][e] * xh[i][e]; ab[i][e] += d[i][e]; }
-        d[i][e] *= g[i][e];
-        s1 += d[i][e];
-        s2 += d[i][e] * xh[i][e];
+        const float xh = (to_f32(xc[i][e]) - mean) * rstd, d = to_f32(dc[i][e]);       // columns past C and dead rows: d = 0
+        if (WG) { ag[i][e] += d * xh; ab[i][e] += d; }
+        const float gd = d * g[i][e];
+        s1 += gd;
+        s2 += gd * xh;
       }
     s1 = row_sum<LPR>(s1, red, slot) * rC;
     s2 = row_sum<LPR>(s2, red, slot + 1) * rC;
     slot ^= 2;
-    if (live) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) asm("" : "+v"(xc[i]), "+v"(dc[i]));      // convert again: keeping the fp32 values costs 16 registers per vector
+    if (row < rows) {
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
         const int vi = sub + LPR * i;
         if (vi < nvec) {
           float o[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = st.y * (d[i][e] - s1 - xh[i][e] * s2);
-          st_row8<T, AL>(dx + rr * lddx, vi * 8, C, o);
+          for (int e = 0; e < 8; ++e) {
+            const float xh = (to_f32(xc[i][e]) - mean) * rstd;
+            o[e] = rstd * (to_f32(dc[i][e]) * g[i][e] - s1 - xh * s2);
+          }
+          st_row8<T, AL>(dx + row * lddx, vi * 8, C, o);
         }
       }
     }
@@ -213,32 +238,37 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* dy, long ldd, cons
   }
 }
 
-// sums[c] = sum over the workgroups' parts, in order: 16 columns x 16 part groups per workgroup
-__global__ __launch_bounds__(256) void ln_bwd_join_kernel(const float* __restrict__ parts, int nparts, int C, float* dgamma, float* dbeta) {
-  __shared__ float sm[16][17];
+// sums[c] = sum over the workgroups' parts, in order: 16 columns x 64 part groups per workgroup
+__global__ __launch_bounds__(1024) void ln_bwd_join_kernel(const float* __restrict__ parts, int nparts, int C, float* dgamma, float* dbeta) {
+  __shared__ float sm[64][17];
   const int cl = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const int c = blockIdx.x * 16 + cl;
   float s = 0.0f;
   if (c < 2 * C)
-    for (int p = grp; p < nparts; p += 16) s += parts[(long)p * 2 * C + c];
+#pragma unroll 4
+    for (int p = grp; p < nparts; p += 64) s += parts[(long)p * 2 * C + c];
   sm[grp][cl] = s;
   __syncthreads();
-  if (grp == 0 && c < 2 * C) {
+  if (grp >= 4) return;
+  float t = 0.0f;
 #pragma unroll
-    for (int k = 1; k < 16; ++k) s += sm[k][cl];
-    if (c < C) dgamma[c] = s; else dbeta[c - C] = s;
+  for (int k = 0; k < 16; ++k) t += sm[grp * 16 + k][cl];
+  sm[grp * 16][cl] = t;                          // row grp * 16 is read by this thread alone
+  __builtin_amdgcn_wave_barrier();               // the four groups are one wave
+  if (grp == 0 && c < 2 * C) {
+    t = (sm[0][cl] + sm[16][cl]) + (sm[32][cl] + sm[48][cl]);
+    if (c < C) dgamma[c] = t; else dbeta[c - C] = t;
   }
 }
 
-// lanes per row and vectors per lane for a row of nvec vectors: the fewest lanes that hold it with at most 5 vectors each (5: the
-// widest lane whose backward pass -- x, dy, gamma, two gradients in fp32 -- still leaves two waves per SIMD), past 320 vectors the workgroup
+// Lanes per row and vectors per lane for a row of nvec vectors: the fewest lanes that hold it with at most 3 vectors each, past 192
+// vectors the whole workgroup.  3 is for the backward pass -- x and dy twice (now and next), gamma and both gradients in registers --
+// on 262144 rows of 320 (bf16): 16 lanes x 3 (a sixth of them idle) 107 us, 8 lanes x 5 (none idle, one wave per SIMD) 147 us.
 void pick(int nvec, bool al, int& lpr, int& vpl) {
-  if (nvec > 320) { lpr = 256; vpl = nvec <= 512 ? 2 : (nvec <= 1024 ? 4 : 8); return; }
+  if (nvec > 192) { lpr = 256; vpl = nvec <= 512 ? 2 : (nvec <= 1024 ? 4 : 8); return; }
   lpr = 8;
-  while (lpr * 5 < nvec) lpr *= 2;
-  vpl = (nvec + lpr - 1) / lpr;
-  if (!al) vpl = 5;                              // rows that are not 16-byte aligned: one form per lane count
-  else if (lpr > 8 && vpl < 3) vpl = 3;
+  while (lpr * 3 < nvec) lpr *= 2;
+  vpl = lpr > 8 || !al ? 3 : (nvec + lpr - 1) / lpr;       // rows that are not 16-byte aligned: one form per lane count
 }
 
 constexpr int LN_MAX_C = 16384;
@@ -246,15 +276,7 @@ constexpr int LN_BWD_WGS = 1024;                 // workgroups of the backward p
 
 template <typename F> int with_shape(int lpr, int vpl, F&& f) {
 #define CASE(L, V) if (lpr == L && vpl == V) return f(std::integral_constant<int, L>{}, std::integral_constant<int, V>{});
-  CASE(8, 1) CASE(8, 2) CASE(8, 3) CASE(8, 4) CASE(8, 5)
-  CASE(16, 3) CASE(16, 4) CASE(16, 5) CASE(32, 3) CASE(32, 4) CASE(32, 5) CASE(64, 3) CASE(64, 4) CASE(64, 5)
-  CASE(256, 2) CASE(256, 4) CASE(256, 8)
-#undef CASE
-  return -22;
-}
-template <typename F> int with_shape_u(int lpr, int vpl, F&& f) {
-#define CASE(L, V) if (lpr == L && vpl == V) return f(std::integral_constant<int, L>{}, std::integral_constant<int, V>{});
-  CASE(8, 5) CASE(16, 5) CASE(32, 5) CASE(64, 5) CASE(256, 2) CASE(256, 4) CASE(256, 8)
+  CASE(8, 1) CASE(8, 2) CASE(8, 3) CASE(16, 3) CASE(32, 3) CASE(64, 3) CASE(256, 2) CASE(256, 4) CASE(256, 8)
 #undef CASE
   return -22;
 }
@@ -276,7 +298,7 @@ int launch_fwd(const void* x, int64_t ldx, void* y, int64_t ldy, const void* g, 
     return 0;
   };
   return al ? with_shape(lpr, vpl, [&](auto L, auto V) { return go(L, V, std::true_type{}); })
-            : with_shape_u(lpr, vpl, [&](auto L, auto V) { return go(L, V, std::false_type{}); });
+            : with_shape(lpr, vpl, [&](auto L, auto V) { return go(L, V, std::false_type{}); });
 }
 
 int bwd_wgs(int64_t rows, int lpr) {
@@ -304,13 +326,13 @@ int launch_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const fl
   if (wgs > 0) {
     auto al_go = [&](auto W) {
       return al ? with_shape(lpr, vpl, [&](auto L, auto V) { return go(L, V, std::true_type{}, W); })
-                : with_shape_u(lpr, vpl, [&](auto L, auto V) { return go(L, V, std::false_type{}, W); });
+                : with_shape(lpr, vpl, [&](auto L, auto V) { return go(L, V, std::false_type{}, W); });
     };
     const int rc = dgamma ? al_go(std::true_type{}) : al_go(std::false_type{});
     if (rc) return rc;
   }
   if (dgamma && !direct) {
-    hipLaunchKernelGGL(ln_bwd_join_kernel, dim3((2 * C + 15) / 16), dim3(256), 0, st, parts, wgs, C, dgamma, dbeta);
+    hipLaunchKernelGGL(ln_bwd_join_kernel, dim3((2 * C + 15) / 16), dim3(1024), 0, st, parts, wgs, C, dgamma, dbeta);
     HALLO_CHECK_LAUNCH();
   }
   return 0;

@@ -9,7 +9,8 @@
 //
 // The kernel is bound by HBM (x read once, y written once).  A workgroup takes `tt` tokens: it computes their cos / sin once into LDS,
 // shared by all heads, then walks (token, head, unit); a unit is V columns and, in the half-split form, their V partners, so every
-// element is read and written by one thread (y may be x).  V = the largest of 8, 4, 2, 1 that divides the axes' (half) widths.
+// element is read and written by one thread (y may be x).  V = 8 or 4, whichever divides the axes' (half) widths; other widths go
+// through rope_staged_kernel.
 #include "common.h"
 #include "../../include/hallo_amd.h"
 
@@ -27,41 +28,13 @@ struct RopeArgs {
   const unsigned long long* freq;                // [pairs] turns * 2^64
   const int* pos; long pos_bs;                   // [B or 1, L, n_axes]; null: grid
   int n_axes, dims[4], grid[4], origin[4];
-  int inverse, heads, hd, pairs, tt;
+  int inverse, heads, hd, pairs, tt, hb;         // hb: heads of a staged tile
   long L, tokens;                                // tokens = B * L
 };
 
-template <typename T, int V> struct __attribute__((aligned(2 * V))) PieceA { T v[V]; };
-template <typename T, int V> struct __attribute__((packed, aligned(2))) PieceU { T v[V]; };
-
-// IL: interleaved pairs.  AL: every piece of V columns is aligned to its size.
-template <typename T, int V, bool IL, bool AL>
-__global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
-  using P = typename std::conditional<AL, PieceA<T, V>, PieceU<T, V>>::type;
-  __shared__ float2 cs[ROPE_PAIRS];
-  __shared__ int ucol[ROPE_MAX_HD], upart[ROPE_MAX_HD], upair[ROPE_MAX_HD];    // unit: first column, partner column (-1: passes through), first pair
-  __shared__ long xoff[ROPE_TT], yoff[ROPE_TT];
+// row offsets, and cos / sin of every pair, of the workgroup's tokens t0 .. t0 + nt - 1
+__device__ __forceinline__ void rope_angles(const RopeArgs& p, long t0, int nt, float2* cs, long* xoff, long* yoff) {
   const int tid = threadIdx.x;
-  const long t0 = (long)blockIdx.x * p.tt;
-  const int nt = (int)(p.tokens - t0 < p.tt ? p.tokens - t0 : p.tt);
-
-  // unit table (the axes' sections, then the columns that pass through)
-  int units = 0;
-  {
-    int col = 0, pair = 0;
-    for (int a = 0; a < p.n_axes; ++a) {
-      const int d = p.dims[a], n = (IL ? d : d / 2) / V;
-      for (int u = tid; u < n; u += 256) {
-        ucol[units + u] = col + u * V;
-        upart[units + u] = IL ? 0 : col + d / 2 + u * V;
-        upair[units + u] = pair + (IL ? u * V / 2 : u * V);
-      }
-      units += n; col += d; pair += d / 2;
-    }
-    const int n = (p.hd - col) / V;
-    for (int u = tid; u < n; u += 256) { ucol[units + u] = col + u * V; upart[units + u] = -1; upair[units + u] = 0; }
-    if (p.x != p.y) units += n;                  // in place they stay where they are
-  }
   if (tid < nt) {
     const long t = t0 + tid, b = t / p.L, l = t - b * p.L;
     xoff[tid] = b * p.x_bs + l * p.x_rs;
@@ -85,6 +58,40 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
     sincospif(half_turns, &s, &c);
     cs[k] = make_float2(c, p.inverse ? -s : s);
   }
+}
+
+template <typename T, int V> struct __attribute__((aligned(2 * V))) PieceA { T v[V]; };
+template <typename T, int V> struct __attribute__((packed, aligned(2))) PieceU { T v[V]; };
+
+// IL: interleaved pairs.  AL: every piece of V columns is aligned to its size.
+template <typename T, int V, bool IL, bool AL>
+__global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
+  using P = typename std::conditional<AL, PieceA<T, V>, PieceU<T, V>>::type;
+  __shared__ float2 cs[ROPE_PAIRS];
+  __shared__ int ucol[ROPE_MAX_HD / 4], upart[ROPE_MAX_HD / 4], upair[ROPE_MAX_HD / 4];    // unit: first column, partner column (-1: passes through), first pair
+  __shared__ long xoff[ROPE_TT], yoff[ROPE_TT];
+  const int tid = threadIdx.x;
+  const long t0 = (long)blockIdx.x * p.tt;
+  const int nt = (int)(p.tokens - t0 < p.tt ? p.tokens - t0 : p.tt);
+
+  // unit table (the axes' sections, then the columns that pass through)
+  int units = 0;
+  {
+    int col = 0, pair = 0;
+    for (int a = 0; a < p.n_axes; ++a) {
+      const int d = p.dims[a], n = (IL ? d : d / 2) / V;
+      for (int u = tid; u < n; u += 256) {
+        ucol[units + u] = col + u * V;
+        upart[units + u] = IL ? 0 : col + d / 2 + u * V;
+        upair[units + u] = pair + (IL ? u * V / 2 : u * V);
+      }
+      units += n; col += d; pair += d / 2;
+    }
+    const int n = (p.hd - col) / V;
+    for (int u = tid; u < n; u += 256) { ucol[units + u] = col + u * V; upart[units + u] = -1; upair[units + u] = 0; }
+    if (p.x != p.y) units += n;                  // in place they stay where they are
+  }
+  rope_angles(p, t0, nt, cs, xoff, yoff);
   __syncthreads();
 
   const T* X = reinterpret_cast<const T*>(p.x);
@@ -139,6 +146,79 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
   }
 }
 
+// Axes whose (half) widths are odd or twice odd: pieces of 1 or 2 columns would be all address arithmetic.  Here whole rows go through
+// LDS in 16-byte chunks (the last one of a row of odd width element by element), and a thread turns the 8 columns of its chunk with the
+// partner columns read from LDS.
+constexpr int ROPE_STAGE = 8192;                 // elements of the staged tile (16 KB)
+
+template <typename T, bool AL>
+__global__ __launch_bounds__(256) void rope_staged_kernel(const RopeArgs p, int il) {
+  using V8 = typename Vec<T>::v8;
+  struct __attribute__((packed, aligned(2))) Loose { V8 v; };
+  __shared__ float2 cs[ROPE_PAIRS];
+  __shared__ __attribute__((aligned(16))) T tile[ROPE_STAGE + 8 * ROPE_TT];
+  __shared__ int map[ROPE_MAX_HD];               // column -> partner - column, pair, sign of sin (0: passes through)
+  __shared__ long xoff[ROPE_TT], yoff[ROPE_TT];
+  const int tid = threadIdx.x;
+  const long t0 = (long)blockIdx.x * p.tt;
+  const int nt = (int)(p.tokens - t0 < p.tt ? p.tokens - t0 : p.tt);
+  for (int c = tid; c < p.hd; c += 256) {
+    int at = 0, pair = 0, a = 0, v = 0;
+    while (a < p.n_axes && c >= at + p.dims[a]) { at += p.dims[a]; pair += p.dims[a] / 2; ++a; }
+    if (a < p.n_axes) {
+      const int i = c - at, half = p.dims[a] / 2, up = il ? i & 1 : i >= half, step = il ? 1 : half;
+      v = (up ? -step : step) * 65536 + (pair + (il ? i >> 1 : i - up * half)) * 4 + (up ? 1 : 2);
+    }
+    map[c] = v;
+  }
+  rope_angles(p, t0, nt, cs, xoff, yoff);
+  __syncthreads();
+  const T* X = reinterpret_cast<const T*>(p.x);
+  T* Y = reinterpret_cast<T*>(p.y);
+  const int hb = p.hb;
+  for (int h0 = 0; h0 < p.heads; h0 += hb) {
+    const int width = min(hb, p.heads - h0) * p.hd, nch = (width + 7) / 8;
+    const long base = (long)h0 * p.hd;
+    for (int k = tid; k < nt * nch; k += 256) {
+      const int t = k / nch, c = (k - t * nch) * 8;
+      const T* xr = X + xoff[t] + base + c;
+      V8 v = zero8<T>();
+      if (c + 8 <= width) v = AL ? ld8<T>(xr) : reinterpret_cast<const Loose*>(xr)->v;
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < width) v[e] = xr[e];
+      st8<T>(tile + t * nch * 8 + c, v);
+    }
+    __syncthreads();
+    for (int k = tid; k < nt * nch; k += 256) {
+      const int t = k / nch, c = (k - t * nch) * 8;
+      const T* row = tile + t * nch * 8;
+      const V8 v = ld8<T>(row + c);
+      const float2* w = cs + t * p.pairs;
+      V8 o;
+      int col = c % p.hd;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int m = c + e < width ? map[col] : 0;
+        const float2 f = w[(m & 0xffff) >> 2];
+        const float s = m & 1 ? f.y : -f.y;
+        o[e] = m ? from_f32<T>(to_f32(v[e]) * f.x + to_f32(row[c + e + (m >> 16)]) * s) : v[e];
+        if (++col == p.hd) col = 0;
+      }
+      T* yr = Y + yoff[t] + base + c;
+      if (c + 8 <= width) {
+        if (AL) st8<T>(yr, o);
+        else reinterpret_cast<Loose*>(yr)->v = o;
+      } else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < width) yr[e] = o[e];
+    }
+    __syncthreads();
+  }
+}
+
 template <typename T, int V, bool IL>
 int launch_rope(const RopeArgs& a, bool al, hipStream_t st) {
   const long grid = (a.tokens + a.tt - 1) / a.tt;
@@ -150,10 +230,19 @@ int launch_rope(const RopeArgs& a, bool al, hipStream_t st) {
 }
 
 template <typename T>
+int launch_staged(const RopeArgs& a, bool il, bool al, hipStream_t st) {
+  const long grid = (a.tokens + a.tt - 1) / a.tt;
+  if (grid > 0x7fffffff) return -22;
+  if (al) hipLaunchKernelGGL((rope_staged_kernel<T, true>), dim3((unsigned)grid), dim3(256), 0, st, a, (int)il);
+  else hipLaunchKernelGGL((rope_staged_kernel<T, false>), dim3((unsigned)grid), dim3(256), 0, st, a, (int)il);
+  HALLO_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
 int pick_rope(const RopeArgs& a, int V, bool il, bool al, hipStream_t st) {
-  if (il) return V == 8 ? launch_rope<T, 8, true>(a, al, st) : V == 4 ? launch_rope<T, 4, true>(a, al, st) : launch_rope<T, 2, true>(a, al, st);
-  return V == 8 ? launch_rope<T, 8, false>(a, al, st)
-                : V == 4 ? launch_rope<T, 4, false>(a, al, st) : V == 2 ? launch_rope<T, 2, false>(a, al, st) : launch_rope<T, 1, false>(a, al, st);
+  if (il) return V == 8 ? launch_rope<T, 8, true>(a, al, st) : launch_rope<T, 4, true>(a, al, st);
+  return V == 8 ? launch_rope<T, 8, false>(a, al, st) : launch_rope<T, 4, false>(a, al, st);
 }
 
 }  // namespace
@@ -197,12 +286,24 @@ extern "C" int hallo_rope(const hallo_rope_desc* d, void* stream) {
   const int V = g % 8 == 0 ? 8 : g % 4 == 0 ? 4 : g % 2 == 0 ? 2 : 1;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) |
                          (uintptr_t)(2 * (a.x_rs | a.y_rs | a.hd | (d->batch > 1 ? a.x_bs | a.y_bs : 0)));
-  const bool al = bits % (2 * V) == 0;
   // tokens of a workgroup: enough to fill its lanes and the cos / sin table, few enough to spread over the 256 CUs
+  // pieces of 4 columns: 150 us direct, 214 us staged (262144 tokens, 16 heads of 40); pieces of 1: 26 us direct, under 19 us staged (8510
+  // tokens, 16 heads of 80)
+  const bool staged = V <= 2;
   int tt = ROPE_PAIRS / a.pairs;
   if (tt > ROPE_TT) tt = ROPE_TT;
+  if (staged && tt * a.hd > ROPE_STAGE) tt = ROPE_STAGE / a.hd;
   while (tt > 1 && (a.tokens + tt - 1) / tt < 1024) tt = (tt + 1) / 2;
   a.tt = tt;
   hipStream_t st = (hipStream_t)stream;
+  if (staged) {
+    a.hb = ROPE_STAGE / (tt * a.hd);
+    if (a.hb >= a.heads) a.hb = a.heads;
+    else if (a.hb >= 8) a.hb = a.hb / 8 * 8;     // later tiles start at multiples of 8 columns
+    const uintptr_t rows = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) |
+                           (uintptr_t)(2 * (a.x_rs | a.y_rs | (d->batch > 1 ? a.x_bs | a.y_bs : 0) | (a.hb < a.heads ? a.hb * a.hd : 0)));
+    return d->dtype == DT_F16 ? launch_staged<_Float16>(a, il, rows % 16 == 0, st) : launch_staged<__bf16>(a, il, rows % 16 == 0, st);
+  }
+  const bool al = bits % (2 * V) == 0;
   return d->dtype == DT_F16 ? pick_rope<_Float16>(a, V, il, al, st) : pick_rope<__bf16>(a, V, il, al, st);
 }

@@ -856,59 +856,60 @@ def lerp_rows(x, out_rows):
 
 # ---- transformer-block operators with gradients: LayerNorm, rotary positions, window attention -------------------------------------
 # Their workspaces are allocated per call: a captured graph gets them from its own pool, so two graphs never share one, and the
-# allocator orders the reuse of a freed one on its stream.
+# allocator orders the reuse of a freed one on its stream.  Single tokens and short rows are host-bound, so messages are only put
+# together where a call is refused.
 
-class _on:
-    """The stream to launch on for tensors of `t`'s device -- that device's current stream, with the device made current for the
-    launch when another one is (a stream only takes launches from its own device)."""
-
-    def __init__(self, t):
-        self.device = t.device
-        self._guard = None
-
-    def __enter__(self):
-        if self.device.index != torch.cuda.current_device():
-            self._guard = torch.cuda.device(self.device)
-            self._guard.__enter__()
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-        return False
+def _bad(what):
+    raise _l.HalloLibraryError(what)
 
 
-def _need(ok, what):
-    if not ok:
-        raise _l.HalloLibraryError(what)
+def _call(name, device, *args):
+    """One library call on `device`'s current stream, with the device made current for the launch when another one is (a stream only
+    takes launches from its own device)."""
+    fn = getattr(_l.load(), name)
+    i = device.index
+    if i == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if status:
+        _l.check(status, name)
 
 
-def _same(name, t, like, dtype=None):
-    """`t` is on `like`'s device and of its type (or `dtype`)."""
-    _need(t.device == like.device, f"{name} is on {t.device}, expected {like.device}")
-    _need(t.dtype == (dtype or like.dtype), f"{name} is {t.dtype}, expected {dtype or like.dtype}")
+def _like(name, t, like, dtype=None, shape=True):
+    """`t` is on `like`'s device, of its type (or `dtype`) and, with `shape`, of its shape."""
+    if t.device != like.device:
+        _bad(f"{name} is on {t.device}, expected {like.device}")
+    if t.dtype != (dtype or like.dtype):
+        _bad(f"{name} is {t.dtype}, expected {dtype or like.dtype}")
+    if shape and t.shape != like.shape:
+        _bad(f"{name}: expected {tuple(like.shape)}, got {tuple(t.shape)}")
 
 
 def _rows2d(name, x):
     """x [..., C] as (rows, C, row pitch): contiguous, or a 2-D view with contiguous rows."""
-    _need(x.dim() >= 1 and x.shape[-1] >= 1, f"{name}: expected [..., C] with C >= 1, got {tuple(x.shape)}")
-    Cd = x.shape[-1]
-    if x.is_contiguous() or x.numel() == 0:
-        return x.numel() // Cd, Cd, Cd
-    _need(x.dim() == 2 and (x.stride(1) == 1 or Cd == 1) and (x.stride(0) >= Cd or x.shape[0] == 1),
-          f"{name}: expected a contiguous tensor or a 2-D view with contiguous rows, got shape {tuple(x.shape)} strides {x.stride()}")
-    return x.shape[0], Cd, max(x.stride(0), Cd)
+    sh = x.shape
+    if not sh or sh[-1] < 1:
+        _bad(f"{name}: expected [..., C] with C >= 1, got {tuple(sh)}")
+    Cd, n = sh[-1], x.numel()
+    if n == 0 or x.is_contiguous():
+        return n // Cd, Cd, Cd
+    st = x.stride()
+    if len(sh) != 2 or (st[1] != 1 and Cd > 1) or (st[0] < Cd and sh[0] > 1):
+        _bad(f"{name}: expected a contiguous tensor or a 2-D view with contiguous rows, got shape {tuple(sh)} strides {st}")
+    return sh[0], Cd, max(st[0], Cd)
 
 
 def _affine(x, gamma, beta):
     """Checks gamma / beta [C] (x's type or fp32, the same for both); returns the library's affine_f32 flag."""
-    ws = [w for w in (gamma, beta) if w is not None]
     for name, w in (("gamma", gamma), ("beta", beta)):
-        if w is not None:
-            _need(w.device == x.device and w.dtype in (x.dtype, torch.float32) and w.is_contiguous() and w.numel() == x.shape[-1],
-                  f"{name}: expected [{x.shape[-1]}] of {x.dtype} or float32 on {x.device}, got {tuple(w.shape)} {w.dtype} on {w.device}")
-    _need(len({w.dtype for w in ws}) <= 1, "gamma and beta have different types")
-    return 1 if ws and ws[0].dtype == torch.float32 else 0
+        if w is not None and (w.device != x.device or w.dtype not in (x.dtype, torch.float32) or w.shape != x.shape[-1:] or not w.is_contiguous()):
+            _bad(f"{name}: expected contiguous [{x.shape[-1]}] of {x.dtype} or float32 on {x.device}, got {tuple(w.shape)} {w.dtype} on {w.device}")
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        _bad("gamma and beta have different types")
+    w = beta if gamma is None else gamma
+    return 1 if w is not None and w.dtype == torch.float32 else 0
 
 
 def layernorm_train(x, gamma=None, beta=None, eps=1e-5, *, out=None):
@@ -919,14 +920,13 @@ def layernorm_train(x, gamma=None, beta=None, eps=1e-5, *, out=None):
     rows, Cd, ldx = _rows2d("x", x)
     f32 = _affine(x, gamma, beta)
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    _same("out", out, x)
-    _need(out.shape == x.shape, f"out: expected {tuple(x.shape)}, got {tuple(out.shape)}")
+        out = torch.empty_like(x)
+    else:
+        _like("out", out, x)
     ldy = _rows2d("out", out)[2]
     stats = torch.empty((rows, 2), device=x.device, dtype=torch.float32)
-    with _on(x) as st:
-        _l.check(_l.load().hallo_layernorm_train(_p(x), ldx, _p(out), ldy, _p(gamma), _p(beta), f32, _p(stats), rows, Cd, float(eps), code,
-                                                 st), "hallo_layernorm_train")
+    _call("hallo_layernorm_train", x.device, x.data_ptr(), ldx, out.data_ptr(), ldy, gamma.data_ptr() if gamma is not None else None,
+          beta.data_ptr() if beta is not None else None, f32, stats.data_ptr(), rows, Cd, float(eps), code)
     return out, stats
 
 
@@ -936,30 +936,31 @@ def layernorm_backward(dy, x, stats, gamma=None, *, weight_grads=True, out=None)
     _chk_dev(dy, x, stats, gamma, out)
     code = dtype_code(x.dtype)
     rows, Cd, ldx = _rows2d("x", x)
-    _same("dy", dy, x)
-    _need(dy.shape == x.shape, f"dy: expected {tuple(x.shape)}, got {tuple(dy.shape)}")
+    _like("dy", dy, x)
     ldd = _rows2d("dy", dy)[2]
-    _same("stats", stats, x, torch.float32)
-    _need(stats.is_contiguous() and stats.shape == (rows, 2), f"stats: expected contiguous ({rows}, 2), got {tuple(stats.shape)}")
+    _like("stats", stats, x, torch.float32, False)
+    if stats.shape != (rows, 2) or not stats.is_contiguous():
+        _bad(f"stats: expected contiguous ({rows}, 2), got {tuple(stats.shape)}")
     f32 = _affine(x, gamma, None)
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    _same("out", out, x)
-    _need(out.shape == x.shape, f"out: expected {tuple(x.shape)}, got {tuple(out.shape)}")
+        out = torch.empty_like(x)
+    else:
+        _like("out", out, x)
     ldo = _rows2d("out", out)[2]
-    lib = _l.load()
-    wg = ws = None
+    dg = db = pg = pb = pw = None
     need = 0
     if weight_grads:
+        need = _l.load().hallo_layernorm_backward_workspace(rows, Cd)
+        if need < 0:
+            _l.check(need, "hallo_layernorm_backward_workspace")
         wg = torch.empty((2, Cd), device=x.device, dtype=torch.float32)
-        need = lib.hallo_layernorm_backward_workspace(rows, Cd)
-        _need(need >= 0, f"hallo_layernorm_backward_workspace({rows}, {Cd}) failed with status {need}")
-        ws = torch.empty(max(need // 4, 1), device=x.device, dtype=torch.float32)
-    with _on(x) as st:
-        _l.check(lib.hallo_layernorm_backward(_p(dy), ldd, _p(x), ldx, _p(stats), _p(gamma), f32, _p(out), ldo,
-                                              _p(wg[0]) if weight_grads else None, _p(wg[1]) if weight_grads else None, _p(ws), need, rows,
-                                              Cd, code, st), "hallo_layernorm_backward")
-    return (out, wg[0], wg[1]) if weight_grads else (out, None, None)
+        ws = torch.empty(need // 4, device=x.device, dtype=torch.float32)
+        dg, db = wg.unbind(0)
+        pg = wg.data_ptr()
+        pb, pw = pg + 4 * Cd, ws.data_ptr()
+    _call("hallo_layernorm_backward", x.device, dy.data_ptr(), ldd, x.data_ptr(), ldx, stats.data_ptr(),
+          gamma.data_ptr() if gamma is not None else None, f32, out.data_ptr(), ldo, pg, pb, pw, need, rows, Cd, code)
+    return out, dg, db
 
 
 class RopeAxes:
@@ -969,9 +970,12 @@ class RopeAxes:
 
     def __init__(self, dims, head_dim, theta=10000.0, interleaved=False, device="cuda"):
         dims = tuple(int(d) for d in dims)
-        _need(1 <= len(dims) <= 4 and all(d >= 2 and d % 2 == 0 for d in dims), f"dims: expected 1 to 4 even widths, got {dims}")
-        _need(head_dim % 2 == 0 and 2 <= head_dim <= 256 and sum(dims) <= head_dim, f"dims {dims} do not fit head_dim {head_dim} (even, at most 256)")
-        _need(theta > 0 and math.isfinite(theta), f"theta: expected a positive number, got {theta}")
+        if not 1 <= len(dims) <= 4 or any(d < 2 or d % 2 for d in dims):
+            _bad(f"dims: expected 1 to 4 even widths, got {dims}")
+        if head_dim % 2 or not 2 <= head_dim <= 256 or sum(dims) > head_dim:
+            _bad(f"dims {dims} do not fit head_dim {head_dim} (even, at most 256)")
+        if not theta > 0 or not math.isfinite(theta):
+            _bad(f"theta: expected a positive number, got {theta}")
         self.dims, self.head_dim, self.theta, self.interleaved = dims, int(head_dim), float(theta), bool(interleaved)
         turns = [int(round(self.theta ** (-2.0 * i / d) / (2.0 * math.pi) * 2.0 ** 64)) % (1 << 64) for d in dims for i in range(d // 2)]
         self.freq = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64).to(device)
@@ -984,96 +988,113 @@ def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
     `origin` (default 0).  inverse=True turns back: the gradient with respect to x of rope(x) is rope(dy, inverse=True).  out may be x."""
     _chk_dev(x, pos, out, axes.freq)
     code = dtype_code(x.dtype)
-    n = len(axes.dims)
-    _need(x.dim() == 3 and x.shape[2] % axes.head_dim == 0 and x.shape[2] > 0 and x.stride(2) == 1,
-          f"x: expected [B, L, heads * {axes.head_dim}] with contiguous columns, got {tuple(x.shape)} strides {x.stride()}")
-    _need(axes.freq.device == x.device, f"axes were built on {axes.freq.device}, x is on {x.device}")
-    B, L, W = x.shape
+    n, hd, sh, st = len(axes.dims), axes.head_dim, x.shape, x.stride()
+    if len(sh) != 3 or sh[2] % hd or not sh[2] or st[2] != 1:
+        _bad(f"x: expected [B, L, heads * {hd}] with contiguous columns, got {tuple(sh)} strides {st}")
+    if axes.freq.device != x.device:
+        _bad(f"axes were built on {axes.freq.device}, x is on {x.device}")
+    B, L, W = sh
     if out is None:
-        out = torch.empty((B, L, W), device=x.device, dtype=x.dtype)
-    _same("out", out, x)
-    _need(out.shape == x.shape and out.stride(2) == 1 and (L <= 1 or out.stride(1) >= W) and (B <= 1 or L == 0 or out.stride(0) > 0),
-          f"out: expected {tuple(x.shape)} with rows that do not overlap, got {tuple(out.shape)} strides {out.stride()}")
-    _need((pos is None) != (grid is None), "give either pos or grid")
-    d = _l.RopeDesc()
-    d.x, d.y = x.data_ptr(), out.data_ptr()
-    d.x_bs, d.x_rs = (x.stride(0) if B > 1 else 0), (x.stride(1) if L > 1 else W)
-    d.y_bs, d.y_rs = (out.stride(0) if B > 1 else 0), (out.stride(1) if L > 1 else W)
-    d.freq = axes.freq.data_ptr()
+        out = torch.empty_like(x)
+    else:
+        _like("out", out, x)
+    so = out.stride()
+    if so[2] != 1 or (L > 1 and so[1] < W) or (B > 1 and L and not so[0]):
+        _bad(f"out: expected {tuple(sh)} with rows that do not overlap, got {tuple(out.shape)} strides {so}")
+    if (pos is None) == (grid is None):
+        _bad("give either pos or grid")
+    pp, pbs = None, 0
     if pos is not None:
-        _need(origin is None, "origin goes with grid")
-        _same("pos", pos, x, torch.int32)
-        _need(pos.is_contiguous() and tuple(pos.shape) in ((L, n), (B, L, n)), f"pos: expected contiguous ({L}, {n}) or ({B}, {L}, {n}), got {tuple(pos.shape)}")
-        d.pos, d.pos_bs = pos.data_ptr(), (L * n if pos.dim() == 3 else 0)
+        if origin is not None:
+            _bad("origin goes with grid")
+        _like("pos", pos, x, torch.int32, False)
+        if pos.shape == (B, L, n):
+            pbs = L * n
+        elif pos.shape != (L, n):
+            _bad(f"pos: expected contiguous ({L}, {n}) or ({B}, {L}, {n}), got {tuple(pos.shape)}")
+        if not pos.is_contiguous():
+            _bad(f"pos: expected contiguous memory, got strides {pos.stride()}")
+        pp = pos.data_ptr()
+        grid = origin = ()
     else:
         grid, origin = tuple(grid), tuple(origin) if origin is not None else (0,) * n
-        _need(len(grid) == n and len(origin) == n and all(g >= 1 for g in grid) and math.prod(grid) == L,
-              f"grid {grid} (origin {origin}): expected {n} lengths with {L} cells")
-        _need(all(-2 ** 31 <= o and o + g <= 2 ** 31 for o, g in zip(origin, grid)), f"positions from {origin} on pass 32 bits")
-        for i in range(n):
-            d.grid[i], d.origin[i] = grid[i], origin[i]
-        d.pos, d.pos_bs = None, 0
-    for i in range(n):
-        d.dims[i] = axes.dims[i]
-    d.batch, d.L, d.heads, d.head_dim, d.n_axes = B, L, W // axes.head_dim, axes.head_dim, n
-    d.interleaved, d.inverse, d.dtype = int(axes.interleaved), int(bool(inverse)), code
-    with _on(x) as st:
-        _l.check(_l.load().hallo_rope(C.byref(d), st), "hallo_rope")
+        if len(grid) != n or len(origin) != n or min(grid) < 1 or math.prod(grid) != L:
+            _bad(f"grid {grid} (origin {origin}): expected {n} lengths with {L} cells")
+        if any(o < -2 ** 31 or o + g > 2 ** 31 for o, g in zip(origin, grid)):
+            _bad(f"positions from {origin} on pass 32 bits")
+    d = _l.RopeDesc(x.data_ptr(), out.data_ptr(), st[0] if B > 1 else 0, st[1] if L > 1 else W, so[0] if B > 1 else 0, so[1] if L > 1 else W,
+                    axes.freq.data_ptr(), pp, pbs, B, L, W // hd, hd, n, axes.dims, grid, origin, axes.interleaved, bool(inverse), code)
+    _call("hallo_rope", x.device, C.byref(d))
     return out
 
 
-def _heads4(name, t, heads, hd):
+def _heads4(name, t, heads, hd, writable=False):
     """[B, L, heads * hd] or [B, L, heads, hd] view -> its (batch, row, head) strides."""
-    if t.dim() == 3:
-        _need(t.shape[2] == heads * hd, f"{name}: expected [B, L, {heads} * {hd}], got {tuple(t.shape)}")
-        st = (t.stride(0), t.stride(1), hd)
+    sh, st = t.shape, t.stride()
+    if len(sh) == 3:
+        ok = sh[2] == heads * hd and st[2] == 1
+        bs, rs, hs = st[0], st[1], hd
     else:
-        _need(t.dim() == 4 and t.shape[2] == heads and t.shape[3] == hd, f"{name}: expected [B, L, {heads}, {hd}], got {tuple(t.shape)}")
-        st = (t.stride(0), t.stride(1), t.stride(2))
+        ok = len(sh) == 4 and sh[2] == heads and sh[3] == hd and st[3] == 1
+        bs, rs, hs = st[:3] if ok else (0, 0, 0)
+    if not ok:
+        _bad(f"{name}: expected [B, L, {heads} * {hd}] or [B, L, {heads}, {hd}] with contiguous heads, got {tuple(sh)} strides {st}")
+    if writable and ((sh[0] > 1 and not bs) or (sh[1] > 1 and not rs) or (heads > 1 and not hs)):
+        _bad(f"{name}: overlapping rows, strides {st}")
     # strides of single or absent rows, entries and heads never count
-    st = [0 if t.shape[0] <= 1 else st[0], 0 if t.shape[1] <= 1 else st[1], hd if heads == 1 else st[2]]
-    _need(t.stride(-1) == 1 and all(s % 8 == 0 for s in st) and st[1] <= 1 << 24 and (t.data_ptr() % 16 == 0 or t.numel() == 0),
-          f"{name}: expected contiguous head rows, strides that are multiples of 8 (rows at most 2^24 apart) and a 16-byte aligned start, "
-          f"got strides {t.stride()}")
-    return st
+    if sh[0] <= 1:
+        bs = 0
+    if sh[1] <= 1:
+        rs = 0
+    if heads == 1:
+        hs = hd
+    if (bs | rs | hs) & 7 or rs > 1 << 24 or t.data_ptr() & 15:
+        _bad(f"{name}: expected strides that are multiples of 8 (rows at most 2^24 apart) and a 16-byte aligned start, got strides {st}")
+    return bs, rs, hs
 
 
-def _writable(name, t, st):
-    _need(all(s > 0 or n <= 1 for s, n in zip(st, t.shape[:2])) and st[2] > 0, f"{name}: overlapping rows, strides {t.stride()}")
-    return st
+def _edge(n):
+    return -1 if n < 0 else min(int(n), 1 << 29)
 
 
-def _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale):
+def _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, o_written):
+    """(descriptor without workspace, kv_heads, head_dim) of checked arguments."""
     code = dtype_code(q.dtype)
-    _need(heads >= 1, f"heads: {heads}")
-    kv_heads = heads if kv_heads is None else kv_heads
-    _need(kv_heads >= 1 and heads % kv_heads == 0, f"{heads} query heads do not share {kv_heads} key heads")
-    _need(q.dim() in (3, 4) and q.shape[-1] >= 1 and (q.dim() == 4 or q.shape[2] % heads == 0), f"q: expected [B, L, {heads} * head_dim] or 4-D, got {tuple(q.shape)}")
-    hd = q.shape[3] if q.dim() == 4 else q.shape[2] // heads
-    _need(hd % 8 == 0 and 8 <= hd <= 160, f"head_dim {hd}: expected a multiple of 8 up to 160")
-    B, Lq, Lk = q.shape[0], q.shape[1], k.shape[1]
-    _need(Lq <= 1 << 29 and Lk <= 1 << 29, f"lengths {Lq}, {Lk}: at most 2^29")
-    for name, t in (("k", k), ("v", v)):
-        _same(name, t, q)
-        _need(t.dim() in (3, 4) and t.shape[0] == B and t.shape[1] == Lk, f"{name}: expected [{B}, {Lk}, ...], got {tuple(t.shape)}")
+    if kv_heads is None:
+        kv_heads = heads
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        _bad(f"{heads} query heads do not share {kv_heads} key heads")
+    sq, sk = q.shape, k.shape
+    if len(sq) not in (3, 4) or (len(sq) == 3 and sq[2] % heads):
+        _bad(f"q: expected [B, L, {heads} * head_dim] or [B, L, {heads}, head_dim], got {tuple(sq)}")
+    hd = sq[3] if len(sq) == 4 else sq[2] // heads
+    if hd % 8 or not 8 <= hd <= 160:
+        _bad(f"head_dim {hd}: expected a multiple of 8 up to 160")
+    B, Lq = sq[0], sq[1]
+    _like("k", k, q, None, False)
+    _like("v", v, q, None, False)
+    if len(sk) not in (3, 4) or sk[0] != B:
+        _bad(f"k: expected [{B}, L, {kv_heads} * {hd}], got {tuple(sk)}")
+    Lk = sk[1]
+    if v.shape[:2] != sk[:2]:
+        _bad(f"v: expected [{B}, {Lk}, {kv_heads} * {hd}], got {tuple(v.shape)}")
+    if Lq > 1 << 29 or Lk > 1 << 29:
+        _bad(f"lengths {Lq}, {Lk}: at most 2^29")
     for name, t in (("q_len", q_len), ("kv_len", kv_len)):
         if t is not None:
-            _same(name, t, q, torch.int32)
-            _need(t.is_contiguous() and t.shape == (B,), f"{name}: expected contiguous ({B},), got {tuple(t.shape)}")
-    _need(sinks >= 0, f"sinks: {sinks}")
+            _like(name, t, q, torch.int32, False)
+            if t.shape != (B,) or not t.is_contiguous():
+                _bad(f"{name}: expected contiguous ({B},), got {tuple(t.shape)}")
+    if sinks < 0:
+        _bad(f"sinks: {sinks}")
     scale = hd ** -0.5 if scale is None else float(scale)
-    _need(0.0 < scale < 1e30, f"scale: expected a positive number, got {scale}")
-    d = _l.WindowAttnDesc()
-    d.q, d.k, d.v, d.o, d.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), (lse.data_ptr() if lse is not None else None)
-    d.q_bs, d.q_rs, d.q_hs = _heads4("q", q, heads, hd)
-    d.k_bs, d.k_rs, d.k_hs = _heads4("k", k, kv_heads, hd)
-    d.v_bs, d.v_rs, d.v_hs = _heads4("v", v, kv_heads, hd)
-    d.o_bs, d.o_rs, d.o_hs = _heads4("o", o, heads, hd)
-    d.q_len, d.kv_len = (t.data_ptr() if t is not None else None for t in (q_len, kv_len))
-    d.Lq, d.Lk, d.batch, d.heads, d.kv_heads, d.head_dim = Lq, Lk, B, heads, kv_heads, hd
-    edge = lambda n: -1 if n < 0 else min(int(n), 1 << 29)
-    d.left, d.right, d.sinks, d.scale, d.dtype = edge(left), edge(right), edge(sinks), scale, code
-    d.workspace, d.workspace_bytes = None, 0
+    if not 0.0 < scale < 1e30:
+        _bad(f"scale: expected a positive number, got {scale}")
+    d = _l.WindowAttnDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None,
+                          *_heads4("q", q, heads, hd), *_heads4("k", k, kv_heads, hd), *_heads4("v", v, kv_heads, hd),
+                          *_heads4("out" if o_written else "o", o, heads, hd, o_written),
+                          q_len.data_ptr() if q_len is not None else None, kv_len.data_ptr() if kv_len is not None else None,
+                          Lq, Lk, B, heads, kv_heads, hd, _edge(left), _edge(right), _edge(sinks), scale, code)
     return d, kv_heads, hd
 
 
@@ -1091,20 +1112,18 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
     return_lse: (out, lse), lse fp32 [B, heads, Lq] (-inf where nothing is visible), as window_attention_backward() takes it."""
     _chk_dev(q, k, v, q_len, kv_len, out)
     if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    _same("out", out, q)
-    _need(out.shape == q.shape, f"out: expected {tuple(q.shape)}, got {tuple(out.shape)}")
-    lse = torch.empty((q.shape[0], heads, q.shape[1]), device=q.device, dtype=torch.float32) if return_lse else None
-    d, _, hd = _window_desc(q, k, v, out, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale)
-    _writable("out", out, (d.o_bs, d.o_rs, d.o_hs))
-    lib = _l.load()
-    need = lib.hallo_window_attention_workspace(C.byref(d))
-    _need(need >= 0, f"hallo_window_attention_workspace failed with status {need}")
+        out = torch.empty_like(q)
+    else:
+        _like("out", out, q)
+    lse = torch.empty((q.shape[0], heads, q.shape[1]), device=q.device, dtype=torch.float32) if return_lse and heads >= 1 else None
+    d, _, _ = _window_desc(q, k, v, out, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, True)
+    need = _l.load().hallo_window_attention_workspace(C.byref(d))
     if need:
+        if need < 0:
+            _l.check(need, "hallo_window_attention_workspace")
         ws = torch.empty(need // 4, device=q.device, dtype=torch.float32)
         d.workspace, d.workspace_bytes = ws.data_ptr(), need
-    with _on(q) as st:
-        _l.check(lib.hallo_window_attention(C.byref(d), st), "hallo_window_attention")
+    _call("hallo_window_attention", q.device, C.byref(d))
     return (out, lse) if return_lse else out
 
 
@@ -1113,31 +1132,26 @@ def window_attention_backward(do, q, k, v, o, lse, heads, *, kv_heads=None, left
     """(dq, dk, dv) of o, lse = window_attention(q, k, v, ..., return_lse=True) for do, with the same arguments.  dk / dv are summed over
     the query heads that share a key head; padded rows get zeros.  Results repeat bit for bit."""
     _chk_dev(do, q, k, v, o, lse, q_len, kv_len, dq, dk, dv)
-    _same("o", o, q)
-    _same("do", do, q)
-    _same("lse", lse, q, torch.float32)
-    _need(o.shape == q.shape and do.shape == q.shape, f"o, do: expected {tuple(q.shape)}, got {tuple(o.shape)}, {tuple(do.shape)}")
-    _need(lse.is_contiguous() and lse.shape == (q.shape[0], heads, q.shape[1]), f"lse: expected contiguous ({q.shape[0]}, {heads}, {q.shape[1]}), got {tuple(lse.shape)}")
-    w, kv_heads, hd = _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale)
-    d = _l.WindowAttnBwdDesc()
-    d.fwd = w
+    _like("o", o, q)
+    _like("do", do, q)
+    _like("lse", lse, q, torch.float32, False)
+    if lse.shape != (q.shape[0], heads, q.shape[1]) or not lse.is_contiguous():
+        _bad(f"lse: expected contiguous ({q.shape[0]}, {heads}, {q.shape[1]}), got {tuple(lse.shape)}")
+    w, kv_heads, hd = _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, False)
     outs = []
     for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
         if t is None:
             t = torch.empty(like.shape, device=q.device, dtype=q.dtype)
-        _same(name, t, q)
-        _need(t.shape == like.shape, f"{name}: expected {tuple(like.shape)}, got {tuple(t.shape)}")
+        else:
+            _like(name, t, like)
         outs.append(t)
-    d.dout, d.dq, d.dk, d.dv = do.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), outs[2].data_ptr()
-    d.do_bs, d.do_rs, d.do_hs = _heads4("do", do, heads, hd)
-    d.dq_bs, d.dq_rs, d.dq_hs = _writable("dq", outs[0], _heads4("dq", outs[0], heads, hd))
-    d.dk_bs, d.dk_rs, d.dk_hs = _writable("dk", outs[1], _heads4("dk", outs[1], kv_heads, hd))
-    d.dv_bs, d.dv_rs, d.dv_hs = _writable("dv", outs[2], _heads4("dv", outs[2], kv_heads, hd))
-    lib = _l.load()
-    need = lib.hallo_window_attention_backward_workspace(C.byref(d))
-    _need(need >= 0, f"hallo_window_attention_backward_workspace failed with status {need}")
+    dq, dk, dv = outs
+    d = _l.WindowAttnBwdDesc(w, do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *_heads4("do", do, heads, hd),
+                             *_heads4("dq", dq, heads, hd, True), *_heads4("dk", dk, kv_heads, hd, True), *_heads4("dv", dv, kv_heads, hd, True))
+    need = _l.load().hallo_window_attention_backward_workspace(C.byref(d))
+    if need < 0:
+        _l.check(need, "hallo_window_attention_backward_workspace")
     ws = torch.empty(max(need // 4, 4), device=q.device, dtype=torch.float32)
     d.fwd.workspace, d.fwd.workspace_bytes = ws.data_ptr(), need
-    with _on(q) as st:
-        _l.check(lib.hallo_window_attention_backward(C.byref(d), st), "hallo_window_attention_backward")
-    return tuple(outs)
+    _call("hallo_window_attention_backward", q.device, C.byref(d))
+    return dq, dk, dv
