@@ -200,8 +200,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Few queries.  Row r of a block of 32 is query r % Lq of head hk * group + r / Lq.  Bound by the bytes of K and V: a wave reads 32 keys
-// at a time, K straight into MFMA operands (lane = key row), V through an LDS tile of its own (no barrier), the next 32 keys in
-// flight under the products; the four waves take every fourth tile of the split and join through LDS.
+// at a time, whole rows by neighbouring lanes, into LDS tiles of its own (no barrier), the next 32 keys in flight under the products; the four waves take every fourth tile of the split and join through LDS.
 // ------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int HK>
 __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
@@ -209,8 +208,8 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   constexpr int NKS = HK / 16, NDB = (HK + 31) / 32, OP = HK + 4;      // OP: pitch of the joined rows, floats
   constexpr float NEG_INF = -__builtin_inff();
   using Tile = WinTile<HK>;
-  constexpr int VT = 4 * 32 * Tile::PITCH, JT = 32 * OP * 4;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[VT > JT ? VT : JT];
+  constexpr int TB = 32 * Tile::PITCH, WT = 4 * 2 * TB, JT = 32 * OP * 4;      // LDS: K | V of every wave, then the joined rows
+  __shared__ __attribute__((aligned(16))) unsigned char smem[WT > JT ? WT : JT];
   __shared__ float sm_m[4][32], sm_l[4][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, l31 = lane & 31;
@@ -241,16 +240,20 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   const int vhi = !live ? 0 : (p.right < 0 ? kn : min(kn, pos + p.right + 1)), vlo = p.left < 0 ? 0 : pos - p.left;
   const int plo = shift + ilo, phi = shift + ihi;
 
-  V8 kr[NKS], vr[NKS];
+  // lanes along the rows: a load instruction takes whole rows (HK = 128: four rows of 256 bytes)
+  constexpr int CH = HK / 8, U = CH / 2;
+  V8 kr[U], vr[U];
   auto load = [&](int t) {
     const int j0 = t < n0 ? t * 32 : w.s1 + (t - n0) * 32, rem = (t < n0 ? w.e0 : w.e1) - j0;
-    const T* kt = K + (long)(j0 + l31) * p.k_rs + hi * 8;
-    const T* vt = V + (long)(j0 + l31) * p.v_rs + hi * 8;
+    const T* kt = K + (long)j0 * p.k_rs;
+    const T* vt = V + (long)j0 * p.v_rs;
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      const bool ok = l31 < rem && ks * 16 + hi * 8 < p.hd;
-      kr[ks] = ok ? ld8<T>(kt + ks * 16) : zero8<T>();
-      vr[ks] = ok ? ld8<T>(vt + ks * 16) : zero8<T>();
+    for (int i = 0; i < U; ++i) {
+      // 64 % CH == 0: the same lane offset for every i, the rest is uniform
+      const int u = 64 % CH ? lane + 64 * i : lane, r0 = 64 % CH ? 0 : 64 / CH * i, rr = u / CH, ch = u - rr * CH;
+      const bool ok = rr + r0 < rem && ch * 8 < p.hd;
+      kr[i] = ok ? ld8<T>(kt + (long)r0 * p.k_rs + ((unsigned)rr * (unsigned)p.k_rs + ch * 8)) : zero8<T>();
+      vr[i] = ok ? ld8<T>(vt + (long)r0 * p.v_rs + ((unsigned)rr * (unsigned)p.v_rs + ch * 8)) : zero8<T>();
     }
   };
   f32x16 o[NDB];
@@ -260,19 +263,25 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
     for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
   float m = NEG_INF, l = 0.0f;
   const float c = p.c;
-  win_lds* const vt = (win_lds*)smem + wave * 32 * Tile::PITCH;
+  win_lds* const kt = (win_lds*)smem + wave * 2 * TB;
+  win_lds* const vt = kt + TB;
   const Tile tl(lane);
 
   int t = tb + wave;
+  win_loads_done();
   if (t < te) load(t);
   for (; t < te; t += 4) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = lane + 64 * i, rr = u / CH, ch = u - rr * CH;
+      *(__attribute__((address_space(3))) V8*)(kt + Tile::at(rr, ch)) = kr[i];
+      *(__attribute__((address_space(3))) V8*)(vt + Tile::at(rr, ch)) = vr[i];
+    }
+    if (t + 4 < te) load(t + 4);
     f32x16 s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(kr[ks], qf[ks], s);
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) *(__attribute__((address_space(3))) V8*)(vt + tl.along[ks]) = vr[ks];
+    for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(tl.template row<V8>(kt, 0, ks), qf[ks], s);
     const int j0 = t < n0 ? t * 32 : w.s1 + (t - n0) * 32, end = t < n0 ? w.e0 : w.e1;
-    if (t + 4 < te) load(t + 4);
     const bool all = end - j0 >= 32 && (p.right < 0 || j0 + 31 <= plo + p.right) && (p.left < 0 || j0 >= phi - p.left || j0 + 32 <= p.sinks);
     if (!all) {
       const int lhi = min(vhi, end);
@@ -408,7 +417,7 @@ void plan(WinArgs& a) {
   if (keys > a.Lk) keys = a.Lk;
   const long wgs = (long)a.batch * a.kv_heads * a.nrb, tiles = (keys + 31) / 32;
   long ns = (512 + wgs - 1) / wgs;
-  if (ns > tiles / 8) ns = tiles / 8;
+  if (ns > tiles / 4) ns = tiles / 4;            // every wave of a split has a tile
   a.nsplit = ns < 1 ? 1 : (int)ns;
 }
 
