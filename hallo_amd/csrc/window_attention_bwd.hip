@@ -103,18 +103,23 @@ __global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, i
 // Eight waves: four groups of 32 keys times two roles, so that a wave keeps ONE operand and ONE accumulator (HK = 128: 32 + 64
 // registers; both in one wave are 400 registers, and hipcc then moves 128 accumulators between its two register files in every tile) and a
 // SIMD has a wave of each role, whose matrix and vector work overlap.
-//   role 0, tile t:      S = Q K^T, P = exp2(S c - lse2), dV += P^T dO; leaves P (storage type) for its partner in LDS
+//   role 0, tile t:      S = Q K^T, P = exp2(S c - lse2), dV += P^T dO; leaves P for its partner in LDS
 //   role 1, tile t - 1:  dP = dO V^T, dS = P * (dP - delta), dK += dS^T Q
-// Q and dO tiles are kept for two iterations (three LDS stages), P in two, so one barrier per tile is enough.
+// Q and dO tiles are kept for two iterations (three LDS stages), P in two, so one barrier per tile is enough.  P goes over finer than
+// dV's product takes it: dS from the rounded P made dK's error 1.7 times that of one rounding.  It is fp32, except for bf16 rows of 112
+// and 128 columns: there 64 query rows per tile leave room for 16 bits only, and fp16 of P times 2^14 is 8 times as fine as bf16
+// (2 x 8192 tokens, 32 / 8 heads of 128: 3.36 ms; fp32 and 32 query rows per tile: 3.77 ms; P as dV takes it: 3.28 ms).
 template <typename T, int HK>
 __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(const WinBwdArgs a) {
   using V8 = typename Vec<T>::v8;
   constexpr bool F16 = std::is_same<T, _Float16>::value;
-  constexpr int QB = HK <= 64 || HK > 128 ? 32 : 64;     // query rows of a tile: what three stages leave room for
+  constexpr bool HALF_P = !F16 && HK > 96 && HK <= 128, SCALED = F16 || HALF_P;      // SCALED: P is carried times 2^14
+  using PT = typename std::conditional<HALF_P, f16x4, f32x4>::type;
+  constexpr int QB = HK == 80 || HK == 96 || HALF_P ? 64 : 32;     // query rows of a tile: what three stages and P leave room for
   constexpr int NQ = QB / 32, NKS = HK / 16, NDB = (HK + 31) / 32, CH = HK / 8;
   using Tile = WinTile<HK>;
   constexpr int TB = QB * Tile::PITCH, STAGE = 2 * TB + 2 * QB * 4;        // Q | dO | lse2 | delta
-  constexpr int PX = NQ * 2048;                          // P of one key group: NQ x [2][64 lanes] x 16 bytes
+  constexpr int PG = 64 * sizeof(PT), PX = NQ * 4 * PG;  // P of one key group: NQ x [4][64 lanes]
   constexpr int U = (QB * CH + 511) / 512;
   const WinArgs& p = a.w;
   __shared__ __attribute__((aligned(16))) unsigned char smem[3 * STAGE + 2 * 4 * PX];
@@ -222,7 +227,8 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
   // role 0 takes rows of Q and columns of dO, role 1 rows of dO and columns of Q
   const int rfo = role ? TB : 0, tfo = role ? 0 : TB;
   const Tile tl(lane);
-  win_lds* const px = lds + 3 * STAGE + kg * PX + lane * 16;
+  win_lds* const px = lds + 3 * STAGE + kg * PX + lane * (int)sizeof(PT);
+  typedef __attribute__((address_space(3))) PT ldsp;
   const float c = p.c;
 
   if (itb < ite) { load(); store(0); }
@@ -260,7 +266,7 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
           for (int g = 0; g < 4; ++g) {
             const f32x4 ls = *(const __attribute__((address_space(3))) f32x4*)(stat + (n * 32 + 8 * g) * 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * g + e], c, (F16 ? P_EXP : 0.0f) - ls[e]));
+            for (int e = 0; e < 4; ++e) s[n][4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * g + e], c, (SCALED ? P_EXP : 0.0f) - ls[e]));
           }
           if (!all)
 #pragma unroll
@@ -271,22 +277,20 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
 #pragma unroll
           for (int x = 0; x < 16; ++x) f[n][x >> 3][x & 7] = from_f32<T>(s[n][x]);
 #pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2) *(__attribute__((address_space(3))) V8*)(pt + (n * 2 + h2) * 1024) = f[n][h2];
+          for (int g = 0; g < 4; ++g)
+            *(ldsp*)(pt + (n * 4 + g) * PG) = __builtin_convertvector((f32x4{s[n][4 * g], s[n][4 * g + 1], s[n][4 * g + 2], s[n][4 * g + 3]}), PT);
         }
       } else {
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2) {
-            const V8 pv = *(const __attribute__((address_space(3))) V8*)(pt + (n * 2 + h2) * 1024);
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 pv = __builtin_convertvector(*(const ldsp*)(pt + (n * 4 + g) * PG), f32x4);
+            const f32x4 dl = *(const __attribute__((address_space(3))) f32x4*)(stat + (n * 32 + 8 * g) * 4);
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const f32x4 dl = *(const __attribute__((address_space(3))) f32x4*)(stat + (n * 32 + 16 * h2 + 8 * g) * 4);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float dp = s[n][8 * h2 + 4 * g + e] - dl[e];
-                f[n][h2][4 * g + e] = from_f32<T>(to_f32(pv[4 * g + e]) * (F16 ? dp * gs : dp));
-              }
+            for (int e = 0; e < 4; ++e) {
+              const float dp = s[n][4 * g + e] - dl[e];
+              f[n][g >> 1][4 * (g & 1) + e] = from_f32<T>(pv[e] * (F16 ? dp * gs : dp));
             }
           }
       }
@@ -317,7 +321,7 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int kl = kg * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi, j = ka + kl;
-      const float f = role ? (F16 ? sm_g[kl] * p.scale : p.scale) : (F16 ? 0x1p-14f : 1.0f);
+      const float f = role ? (F16 ? sm_g[kl] * p.scale : HALF_P ? p.scale * 0x1p-14f : p.scale) : (SCALED ? 0x1p-14f : 1.0f);
       const float v = j < kb ? acc[db][e] * f : 0.0f;
       if (part) part[(long)kl * 2 * p.hd + d] = v;
       else if (j < kz) D[(long)j * d_rs + d] = from_f32<T>(v);

@@ -6,9 +6,9 @@ Tolerances, per element, u = eps / 2 of the storage type, E = 2^-24, w = |scale|
   o:  P is rounded once for the product (u), sums in fp32 over the keys (n E), one rounding of the result;
       fp16: P below the normal numbers is off by 2^-25 where the row's largest is at least 1;
   dV: the same over the queries, P carried times 2^14 in fp16;
-  dS = P (dP - delta): dP and delta off by (hd + 8) E of their magnitudes, P and dS rounded once each (for dK the product takes the P that
-      dV's took: (1 + u)(1 + u) - 1 = 2 u to first order; fp16: dS to 2^-25 of a scale that is at least 2^14 / (2 |do|_2 |v|_2), norms over
-      the batch entry), then summed against k or q;
+  dS = P (dP - delta): dP and delta off by (hd + 8) E of their magnitudes, dS rounded once (u; fp16: to 2^-25 of a scale that is at least
+      2^14 / (2 |do|_2 |v|_2), norms over the batch entry), then summed against k or q; for dK a bf16 P of 112 and 128 columns is fp16
+      times 2^14 on its way (2^-11 relative, 2^-25 * 2^-14 below the normal numbers);
   fp32 and bf16 results below the smallest normal number, 2^-126, count as 0 (v_exp_f32 and the MFMA operands flush them): a probability is
   off by up to TINY = 2^-126 on top, and so is a bf16 result -- a key whose probabilities are all below it has gradients of 0."""
 import itertools
@@ -101,7 +101,7 @@ class Ref:
         dp = g @ self.v.transpose(2, 3)
         ds = p * (dp - delta)
         e_dp = (hd + 8) * E * (g.abs() @ self.v.abs().transpose(2, 3) + (g * o).abs().sum(3, keepdim=True))
-        e_ds = (2 * u + u * u + 2 * t) * ds.abs() + p * e_dp * (1 + u) ** 2
+        e_ds = (u + 2 * t) * ds.abs() + p * e_dp * (1 + u)
         e_p = (u + 2 * t) * p
         if self.dt == F16:
             norm = 2 * g.norm(dim=3).amax((1, 2)).view(-1, 1, 1, 1) * self.v.norm(dim=3).amax((1, 2)).view(-1, 1, 1, 1)
@@ -109,6 +109,8 @@ class Ref:
             e_p = e_p + 2.0 ** -39 * self.ok
         else:
             e_ds = e_ds + TINY * (1 + (dp - delta).abs()) * self.ok            # P and dS
+            if 96 < hd <= 128:
+                e_ds = e_ds + 2.0 ** -11 * ds.abs() + 2.0 ** -39 * (dp - delta).abs() * self.ok
             e_p = e_p + TINY * self.ok
         nk, nq = self.ok.sum(3, keepdim=True), (self.ok.sum(2).unsqueeze(3) * self.G)
         shared = lambda x: x.reshape(B, Hkv, self.G, Lk, hd).sum(2)
