@@ -62,35 +62,49 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
   const int vhi = p.right < 0 ? kn : min(kn, pos + p.right + 1), vlo = p.left < 0 ? 0 : pos - p.left;
 
   V8 kr[U], vr[U];
-  unsigned ko[U], vo[U];                         // element offsets inside a tile (row strides are at most WIN_MAX_STRIDE)
+  unsigned ko[U], vo[U];                         // byte offsets inside a tile (row strides are at most WIN_MAX_STRIDE)
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
-    ko[i] = (unsigned)rr * (unsigned)p.k_rs + ch * 8;
-    vo[i] = (unsigned)rr * (unsigned)p.v_rs + ch * 8;
+    ko[i] = ((unsigned)rr * (unsigned)p.k_rs + ch * 8) * 2;
+    vo[i] = ((unsigned)rr * (unsigned)p.v_rs + ch * 8) * 2;
   }
+  const bool whole = p.hd == HK;
   auto load = [&](int t) {
     const int j0 = t < n0 ? t * KB : r.s1 + (t - n0) * KB, rem = (t < n0 ? r.e0 : r.e1) - j0;
-    const T* kt = K + (long)j0 * p.k_rs;
-    const T* vt = V + (long)j0 * p.v_rs;
+    const char* kt = reinterpret_cast<const char*>(K + (long)j0 * p.k_rs);
+    const char* vt = reinterpret_cast<const char*>(V + (long)j0 * p.v_rs);
+    if (rem >= KB && whole) {                    // vector instructions do not overlap with the MFMAs here: no masks where none are needed
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
-      const bool ok = rr < rem && rr < KB && ch * 8 < p.hd;        // rows past the range hold anything: they enter the products as zeros
-      kr[i] = ok ? ld8<T>(kt + ko[i]) : zero8<T>();
-      vr[i] = ok ? ld8<T>(vt + vo[i]) : zero8<T>();
+      for (int i = 0; i < U; ++i)
+        if (KB * CH % 256 == 0 || i + 1 < U || tid + 256 * i < KB * CH) {
+          kr[i] = ld8<T>(reinterpret_cast<const T*>(kt + ko[i]));
+          vr[i] = ld8<T>(reinterpret_cast<const T*>(vt + vo[i]));
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+        const bool ok = rr < rem && rr < KB && ch * 8 < p.hd;        // rows past the range hold anything: they enter the products as zeros
+        kr[i] = ok ? ld8<T>(reinterpret_cast<const T*>(kt + ko[i])) : zero8<T>();
+        vr[i] = ok ? ld8<T>(reinterpret_cast<const T*>(vt + vo[i])) : zero8<T>();
+      }
     }
   };
+  int so[U];                                     // this thread's places in a tile
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int u = tid + 256 * i, rr = u / CH;
+    so[i] = Tile::at(rr, u - rr * CH);
+  }
   auto store = [&](int stage) {
     win_lds* const kt = lds + stage * STAGE;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
-      if (KB * CH % 256 == 0 || u < KB * CH) {
-        *(__attribute__((address_space(3))) V8*)(kt + Tile::at(rr, ch)) = kr[i];
-        *(__attribute__((address_space(3))) V8*)(kt + TB + Tile::at(rr, ch)) = vr[i];
+    for (int i = 0; i < U; ++i)
+      if (KB * CH % 256 == 0 || i + 1 < U || tid + 256 * i < KB * CH) {
+        *(__attribute__((address_space(3))) V8*)(kt + so[i]) = kr[i];
+        *(__attribute__((address_space(3))) V8*)(kt + TB + so[i]) = vr[i];
       }
-    }
   };
 
   f32x16 o[NDB];
@@ -107,11 +121,12 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
   win_loads_done();
   if (nt > 1) load(1);
   __syncthreads();
-  for (int t = 0; t < nt; ++t) {
+  auto step = [&](auto odd, int t) {             // odd = t & 1
+    const int P = odd;
     const int j0 = t < n0 ? t * KB : r.s1 + (t - n0) * KB, end = t < n0 ? r.e0 : r.e1;
-    if (t + 1 < nt) store((t + 1) & 1);          // read last in iteration t - 1, which the barrier below closed
+    if (t + 1 < nt) store(1 - P);                // read last in iteration t - 1, which the barrier below closed
     if (t + 2 < nt) load(t + 2);
-    const win_lds* const kt = lds + (t & 1) * STAGE;
+    const win_lds* const kt = lds + P * STAGE;
     const win_lds* const vt = kt + TB;
     const bool none = iw >= qn || (p.right >= 0 && j0 > pw1 + p.right) || (p.left >= 0 && j0 + KB <= pw0 - p.left && j0 >= p.sinks);
     if (!none) {
@@ -174,6 +189,16 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
       win_order<NDB * NT * 2, 2, NDB * NT * 2 < 4 ? 2 : 4>();
     }
     __syncthreads();
+  };
+  if constexpr (HK > 96 && HK <= 128) {          // at the register limit, where two copies of the step cost hipcc its order of the LDS reads
+    for (int t = 0; t < nt; ++t) step(t & 1, t);
+  } else {                                       // the stage as part of the instructions: 2 - 4 % at 64, 80 and 160 columns
+    int t = 0;
+    for (; t + 1 < nt; t += 2) {
+      step(std::integral_constant<int, 0>{}, t);
+      step(std::integral_constant<int, 1>{}, t + 1);
+    }
+    if (t < nt) step(std::integral_constant<int, 0>{}, t);
   }
 
   l = win_half_sum(l);

@@ -62,26 +62,38 @@ __global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, i
   const int h = bid % heads, b = bid / heads;
   const int n = isq ? win_len(p.q_len, b, p.Lq) : win_len(p.kv_len, b, p.Lk);
   float big = 0.0f;
+  V8 xv[4][2], ov[4][2];                         // 16 lanes share a row, a lane's columns are 8 sub and 128 + 8 sub; four rows in flight
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int i = blk * 64 + k * 16 + grp;
+    const T* x = isq ? reinterpret_cast<const T*>(a.dout) + (long)b * a.do_bs + (long)h * a.do_hs + (long)i * a.do_rs
+                     : reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)h * p.v_hs + (long)i * p.v_rs;
+    const T* o = reinterpret_cast<const T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)i * p.o_rs;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int d = sub * 8 + 128 * c;
+      const bool ok = i < n && d < p.hd;
+      xv[k][c] = ok ? ld8<T>(x + d) : zero8<T>();
+      ov[k][c] = ok && isq ? ld8<T>(o + d) : zero8<T>();
+    }
+  }
+#pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int i = blk * 64 + k * 16 + grp;
     float dl = 0.0f, sq = 0.0f;
-    if (i < n) {
-      const T* x = isq ? reinterpret_cast<const T*>(a.dout) + (long)b * a.do_bs + (long)h * a.do_hs + (long)i * a.do_rs
-                       : reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)h * p.v_hs + (long)i * p.v_rs;
-      const T* o = reinterpret_cast<const T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)i * p.o_rs;
-      for (int d = sub * 8; d < p.hd; d += 128) {
-        const V8 xv = ld8<T>(x + d);
-        const V8 ov = isq ? ld8<T>(o + d) : zero8<T>();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float f = to_f32(xv[e]);
-          dl += f * to_f32(ov[e]);
-          sq += f * f;
-        }
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = to_f32(xv[k][c][e]);
+        dl += f * to_f32(ov[k][c][e]);
+        sq += f * f;
       }
-    }
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) { dl += __shfl_xor(dl, s, 64); sq += __shfl_xor(sq, s, 64); }
+    for (int s = 8; s > 0; s >>= 1) {
+      dl += __shfl_xor(dl, s, 64);
+      if (F16) sq += __shfl_xor(sq, s, 64);
+    }
     if (isq && sub == 0 && i < p.Lq) {
       const long at = ((long)b * p.heads + h) * p.Lq + i;
       const float ls = i < n ? p.lse[at] : -__builtin_inff();
@@ -183,17 +195,36 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
 
   V8 qr[U], gr[U];
   float lr = 0.0f, dr = 0.0f;
+  unsigned qo[U], go[U];                         // byte offsets inside a tile, and this thread's places in its LDS image
+  int so[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int u = tid + 512 * i, rr = u / CH, ch = u - rr * CH;
+    qo[i] = ((unsigned)rr * (unsigned)p.q_rs + ch * 8) * 2;
+    go[i] = ((unsigned)rr * (unsigned)a.do_rs + ch * 8) * 2;
+    so[i] = Tile::at(rr, ch);
+  }
+  const bool whole = p.hd == HK;
   int lg = ntq ? itb / ntq : 0, li = itb - lg * ntq;     // head of the group and query tile that load() takes next
   auto load = [&]() {
     const int i0 = ia + li * QB, h = hk * p.group + lg, rem = ib - i0;
-    const T* qt = reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs + (long)i0 * p.q_rs;
-    const T* gt = reinterpret_cast<const T*>(a.dout) + (long)b * a.do_bs + (long)h * a.do_hs + (long)i0 * a.do_rs;
+    const char* qt = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.q) + (long)b * p.q_bs + (long)h * p.q_hs + (long)i0 * p.q_rs);
+    const char* gt = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.dout) + (long)b * a.do_bs + (long)h * a.do_hs + (long)i0 * a.do_rs);
+    if (rem >= QB && whole) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = tid + 512 * i, rr = u / CH, ch = u - rr * CH;
-      const bool ok = rr < rem && rr < QB && ch * 8 < p.hd;
-      qr[i] = ok ? ld8<T>(qt + (unsigned)rr * (unsigned)p.q_rs + ch * 8) : zero8<T>();
-      gr[i] = ok ? ld8<T>(gt + (unsigned)rr * (unsigned)a.do_rs + ch * 8) : zero8<T>();
+      for (int i = 0; i < U; ++i)
+        if (QB * CH % 512 == 0 || i + 1 < U || tid + 512 * i < QB * CH) {
+          qr[i] = ld8<T>(reinterpret_cast<const T*>(qt + qo[i]));
+          gr[i] = ld8<T>(reinterpret_cast<const T*>(gt + go[i]));
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int u = tid + 512 * i, rr = u / CH, ch = u - rr * CH;
+        const bool ok = rr < rem && rr < QB && ch * 8 < p.hd;
+        qr[i] = ok ? ld8<T>(reinterpret_cast<const T*>(qt + qo[i])) : zero8<T>();
+        gr[i] = ok ? ld8<T>(reinterpret_cast<const T*>(gt + go[i])) : zero8<T>();
+      }
     }
     if (tid < QB) {
       const long at = ((long)b * p.heads + h) * p.Lq + i0 + tid;
@@ -205,13 +236,11 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
   auto store = [&](int stage) {
     win_lds* const qt = lds + stage * STAGE;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = tid + 512 * i, rr = u / CH, ch = u - rr * CH;
-      if (QB * CH % 512 == 0 || u < QB * CH) {
-        *(__attribute__((address_space(3))) V8*)(qt + Tile::at(rr, ch)) = qr[i];
-        *(__attribute__((address_space(3))) V8*)(qt + TB + Tile::at(rr, ch)) = gr[i];
+    for (int i = 0; i < U; ++i)
+      if (QB * CH % 512 == 0 || i + 1 < U || tid + 512 * i < QB * CH) {
+        *(__attribute__((address_space(3))) V8*)(qt + so[i]) = qr[i];
+        *(__attribute__((address_space(3))) V8*)(qt + TB + so[i]) = gr[i];
       }
-    }
     if (tid < QB) {
       *(__attribute__((address_space(3))) float*)(qt + 2 * TB + tid * 4) = lr;
       *(__attribute__((address_space(3))) float*)(qt + 2 * TB + QB * 4 + tid * 4) = dr;
@@ -415,28 +444,45 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
   const int vhi = p.right < 0 ? kn : min(kn, pos + p.right + 1), vlo = p.left < 0 ? 0 : pos - p.left;
 
   V8 kr[U], vr[U];
+  unsigned ko[U], vo[U];                         // byte offsets inside a tile, and this thread's places in its LDS image
+  int so[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+    ko[i] = ((unsigned)rr * (unsigned)p.k_rs + ch * 8) * 2;
+    vo[i] = ((unsigned)rr * (unsigned)p.v_rs + ch * 8) * 2;
+    so[i] = Tile::at(rr, ch);
+  }
+  const bool whole = p.hd == HK;
   auto load = [&](int t) {
     const int j0 = t < n0 ? t * KB : r.s1 + (t - n0) * KB, rem = (t < n0 ? r.e0 : r.e1) - j0;
-    const T* kt = K + (long)j0 * p.k_rs;
-    const T* vt = V + (long)j0 * p.v_rs;
+    const char* kt = reinterpret_cast<const char*>(K + (long)j0 * p.k_rs);
+    const char* vt = reinterpret_cast<const char*>(V + (long)j0 * p.v_rs);
+    if (rem >= KB && whole) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
-      const bool ok = rr < rem && rr < KB && ch * 8 < p.hd;
-      kr[i] = ok ? ld8<T>(kt + (unsigned)rr * (unsigned)p.k_rs + ch * 8) : zero8<T>();
-      vr[i] = ok ? ld8<T>(vt + (unsigned)rr * (unsigned)p.v_rs + ch * 8) : zero8<T>();
+      for (int i = 0; i < U; ++i)
+        if (KB * CH % 256 == 0 || i + 1 < U || tid + 256 * i < KB * CH) {
+          kr[i] = ld8<T>(reinterpret_cast<const T*>(kt + ko[i]));
+          vr[i] = ld8<T>(reinterpret_cast<const T*>(vt + vo[i]));
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
+        const bool ok = rr < rem && rr < KB && ch * 8 < p.hd;
+        kr[i] = ok ? ld8<T>(reinterpret_cast<const T*>(kt + ko[i])) : zero8<T>();
+        vr[i] = ok ? ld8<T>(reinterpret_cast<const T*>(vt + vo[i])) : zero8<T>();
+      }
     }
   };
   auto store = [&](int stage) {
     win_lds* const kt = lds + stage * STAGE;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = tid + 256 * i, rr = u / CH, ch = u - rr * CH;
-      if (KB * CH % 256 == 0 || u < KB * CH) {
-        *(__attribute__((address_space(3))) V8*)(kt + Tile::at(rr, ch)) = kr[i];
-        *(__attribute__((address_space(3))) V8*)(kt + TB + Tile::at(rr, ch)) = vr[i];
+    for (int i = 0; i < U; ++i)
+      if (KB * CH % 256 == 0 || i + 1 < U || tid + 256 * i < KB * CH) {
+        *(__attribute__((address_space(3))) V8*)(kt + so[i]) = kr[i];
+        *(__attribute__((address_space(3))) V8*)(kt + TB + so[i]) = vr[i];
       }
-    }
   };
   f32x16 dq[NDB];
 #pragma unroll
@@ -461,9 +507,10 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
     if (!none) {
       f32x16 s = zero16, dp = zero16;
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) s = Vec<T>::mfma32(tl.template row<V8>(kt, 0, ks), qf[ks], s);
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) dp = Vec<T>::mfma32(tl.template row<V8>(vt, 0, ks), gf[ks], dp);
+      for (int ks = 0; ks < NKS; ++ks) {
+        s = Vec<T>::mfma32(tl.template row<V8>(kt, 0, ks), qf[ks], s);
+        dp = Vec<T>::mfma32(tl.template row<V8>(vt, 0, ks), gf[ks], dp);
+      }
       win_order<2 * NKS, 1, NKS < 4 ? NKS : 4>();
       const bool all = end - j0 >= KB && (p.right < 0 || j0 + KB - 1 <= pw0 + p.right) &&
                        (p.left < 0 || j0 >= pw1 - p.left || j0 + KB <= p.sinks);
