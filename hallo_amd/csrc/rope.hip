@@ -32,27 +32,35 @@ struct RopeArgs {
   long L, tokens;                                // tokens = B * L
 };
 
-// row offsets, and cos / sin of every pair, of the workgroup's tokens t0 .. t0 + nt - 1
-__device__ __forceinline__ void rope_angles(const RopeArgs& p, long t0, int nt, float2* cs, long* xoff, long* yoff) {
-  const int tid = threadIdx.x;
-  if (tid < nt) {
-    const long t = t0 + tid, b = t / p.L, l = t - b * p.L;
-    xoff[tid] = b * p.x_bs + l * p.x_rs;
-    yoff[tid] = b * p.y_bs + l * p.y_rs;
+// token t0 + i of the workgroup as (batch entry, place): one long division for t0, 32-bit ones for the rest (L < 2^31)
+struct RopeWhere {
+  long b0; unsigned l0, L;
+  __device__ __forceinline__ RopeWhere(const RopeArgs& p, long t0) : b0(t0 / p.L), l0((unsigned)(t0 - b0 * p.L)), L((unsigned)p.L) {}
+  __device__ __forceinline__ void at(int i, long& b, unsigned& l) const {
+    const unsigned t = l0 + (unsigned)i, q = t / L;
+    b = b0 + q;
+    l = t - q * L;
   }
-  for (int k = tid; k < nt * p.pairs; k += 256) {
+};
+
+// cos / sin of every pair of the workgroup's nt tokens
+__device__ __forceinline__ void rope_angles(const RopeArgs& p, const RopeWhere& where, int nt, float2* cs) {
+  for (int k = threadIdx.x; k < nt * p.pairs; k += 256) {
     const int tt = k / p.pairs, j = k - tt * p.pairs;
-    const long t = t0 + tt, b = t / p.L, l = t - b * p.L;
+    const unsigned long long freq = p.freq[j];
+    long b;
+    unsigned l;
+    where.at(tt, b, l);
     int a = 0, first = 0;
     while (j >= first + p.dims[a] / 2) { first += p.dims[a] / 2; ++a; }
     int pos;
-    if (p.pos) pos = p.pos[b * p.pos_bs + l * p.n_axes + a];
+    if (p.pos) pos = p.pos[b * p.pos_bs + (long)l * p.n_axes + a];
     else {
-      long r = l;
-      for (int c = p.n_axes - 1; c > a; --c) r /= p.grid[c];
-      pos = p.origin[a] + (int)(r % p.grid[a]);
+      unsigned r = l;
+      for (int c = p.n_axes - 1; c > a; --c) r /= (unsigned)p.grid[c];
+      pos = p.origin[a] + (int)(r % (unsigned)p.grid[a]);
     }
-    const unsigned long long turn = (unsigned long long)(long long)pos * p.freq[j];
+    const unsigned long long turn = (unsigned long long)(long long)pos * freq;
     const float half_turns = (float)(int)(unsigned)(turn >> 32) * 0x1p-31f;
     float s, c;
     sincospif(half_turns, &s, &c);
@@ -91,7 +99,15 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
     for (int u = tid; u < n; u += 256) { ucol[units + u] = col + u * V; upart[units + u] = -1; upair[units + u] = 0; }
     if (p.x != p.y) units += n;                  // in place they stay where they are
   }
-  rope_angles(p, t0, nt, cs, xoff, yoff);
+  const RopeWhere where(p, t0);
+  if (tid < nt) {
+    long b;
+    unsigned l;
+    where.at(tid, b, l);
+    xoff[tid] = b * p.x_bs + (long)l * p.x_rs;
+    yoff[tid] = b * p.y_bs + (long)l * p.y_rs;
+  }
+  rope_angles(p, where, nt, cs);
   __syncthreads();
 
   const T* X = reinterpret_cast<const T*>(p.x);
@@ -171,30 +187,82 @@ __global__ __launch_bounds__(256) void rope_staged_kernel(const RopeArgs p, int 
     }
     map[c] = v;
   }
-  rope_angles(p, t0, nt, cs, xoff, yoff);
+  const RopeWhere where(p, t0);
+  if (tid < nt) {
+    long b;
+    unsigned l;
+    where.at(tid, b, l);
+    xoff[tid] = b * p.x_bs + (long)l * p.x_rs;
+    yoff[tid] = b * p.y_bs + (long)l * p.y_rs;
+  }
   __syncthreads();
   const T* X = reinterpret_cast<const T*>(p.x);
   T* Y = reinterpret_cast<T*>(p.y);
-  const int hb = p.hb;
-  for (int h0 = 0; h0 < p.heads; h0 += hb) {
-    const int width = min(hb, p.heads - h0) * p.hd, nch = (width + 7) / 8;
+  constexpr int N = (ROPE_STAGE / 8 + ROPE_TT + 255) / 256;      // chunks of a thread
+  for (int h0 = 0; h0 < p.heads; h0 += p.hb) {
+    const int width = min(p.hb, p.heads - h0) * p.hd, nch = (width + 7) / 8;
     const long base = (long)h0 * p.hd;
-    for (int k = tid; k < nt * nch; k += 256) {
-      const int t = k / nch, c = (k - t * nch) * 8;
-      const T* xr = X + xoff[t] + base + c;
-      V8 v = zero8<T>();
-      if (c + 8 <= width) v = AL ? ld8<T>(xr) : reinterpret_cast<const Loose*>(xr)->v;
-      else
+    V8 in[N];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < width) v[e] = xr[e];
-      st8<T>(tile + t * nch * 8 + c, v);
+    for (int i = 0; i < N; ++i) {
+      const int k = tid + 256 * i, t = k / nch, c = (k - t * nch) * 8;
+      if (k < nt * nch) {
+        const T* xr = X + xoff[t] + base + c;
+        if (c + 8 <= width) in[i] = AL ? ld8<T>(xr) : reinterpret_cast<const Loose*>(xr)->v;
+        else {
+          in[i] = zero8<T>();
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c + e < width) in[i][e] = xr[e];
+        }
+      }
+    }
+    if (h0 == 0) rope_angles(p, where, nt, cs);  // under the first loads
+    else __syncthreads();                        // the tile before this one has been read
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int k = tid + 256 * i;
+      if (k < nt * nch) st8<T>(tile + k * 8, in[i]);
     }
     __syncthreads();
-    for (int k = tid; k < nt * nch; k += 256) {
-      const int t = k / nch, c = (k - t * nch) * 8;
+    if (p.hd % 8 == 0) {
+      // the chunks of a head: a thread keeps the 8 cos, sin and partner distances of its columns over the heads hg, hg + groups, ...
+      const int ncc = p.hd / 8, heads = width / p.hd, groups = max(1, min(heads, 256 / (nt * ncc)));
+      for (int k = tid; k < nt * groups * ncc; k += 256) {
+        const int r = k / ncc, cc = k - r * ncc, t = r / groups, hg = r - t * groups;
+        const float2* w = cs + t * p.pairs;
+        float co[8], si[8];
+        int to[8];
+        unsigned turned = 0;                     // columns of an axis (the others pass through)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int m = map[cc * 8 + e];
+          const float2 f = w[(m & 0xffff) >> 2];
+          co[e] = f.x;
+          si[e] = m & 1 ? f.y : -f.y;
+          to[e] = e + (m >> 16);
+          turned |= (m != 0) << e;
+        }
+        for (int h = hg; h < heads; h += groups) {
+          const T* x = tile + t * nch * 8 + h * p.hd + cc * 8;
+          const V8 v = ld8<T>(x);
+          V8 o = v;
+          if (turned)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (turned >> e & 1) o[e] = from_f32<T>(to_f32(v[e]) * co[e] + to_f32(x[to[e]]) * si[e]);
+          T* yr = Y + yoff[t] + base + h * p.hd + cc * 8;
+          if (AL) st8<T>(yr, o);
+          else reinterpret_cast<Loose*>(yr)->v = o;
+        }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int k = tid + 256 * i, t = k / nch, c = (k - t * nch) * 8;
+      if (k >= nt * nch) break;
       const T* row = tile + t * nch * 8;
-      const V8 v = ld8<T>(row + c);
       const float2* w = cs + t * p.pairs;
       V8 o;
       int col = c % p.hd;
@@ -203,7 +271,7 @@ __global__ __launch_bounds__(256) void rope_staged_kernel(const RopeArgs p, int 
         const int m = c + e < width ? map[col] : 0;
         const float2 f = w[(m & 0xffff) >> 2];
         const float s = m & 1 ? f.y : -f.y;
-        o[e] = m ? from_f32<T>(to_f32(v[e]) * f.x + to_f32(row[c + e + (m >> 16)]) * s) : v[e];
+        o[e] = m ? from_f32<T>(to_f32(in[i][e]) * f.x + to_f32(row[c + e + (m >> 16)]) * s) : in[i][e];
         if (++col == p.hd) col = 0;
       }
       T* yr = Y + yoff[t] + base + c;
@@ -215,7 +283,6 @@ __global__ __launch_bounds__(256) void rope_staged_kernel(const RopeArgs p, int 
         for (int e = 0; e < 8; ++e)
           if (c + e < width) yr[e] = o[e];
     }
-    __syncthreads();
   }
 }
 
@@ -250,7 +317,7 @@ int pick_rope(const RopeArgs& a, int V, bool il, bool al, hipStream_t st) {
 
 extern "C" int hallo_rope(const hallo_rope_desc* d, void* stream) {
   using namespace hallo;
-  if (!d || (d->dtype != DT_F16 && d->dtype != DT_BF16) || d->batch < 0 || d->L < 0 || d->heads < 1 || d->heads > (1 << 20) || d->head_dim < 2 || d->head_dim % 2 ||
+  if (!d || (d->dtype != DT_F16 && d->dtype != DT_BF16) || d->batch < 0 || d->L < 0 || d->heads < 1 || d->heads > (1 << 16) || d->head_dim < 2 || d->head_dim % 2 ||
       d->head_dim > ROPE_MAX_HD || d->n_axes < 1 || d->n_axes > 4 || d->batch > 0x7fffffff)
     return -22;
   RopeArgs a = {};
@@ -273,7 +340,7 @@ extern "C" int hallo_rope(const hallo_rope_desc* d, void* stream) {
   }
   if (sum > d->head_dim || (!d->pos && !none && cells != d->L)) return -22;
   const long width = (long)d->heads * d->head_dim;
-  if (d->x_rs < 0 || d->y_rs < width || d->L > (1L << 40) || (d->batch > 0 && d->L > (1L << 46) / d->batch)) return -22;
+  if (d->x_rs < 0 || d->y_rs < width || d->L > 0x7fffffff - ROPE_TT || (d->batch > 0 && d->L > (1L << 46) / d->batch)) return -22;
   if (none) return 0;
   if (!d->x || !d->y || !d->freq) return -22;
   if (d->x == d->y && (d->x_bs != d->y_bs || d->x_rs != d->y_rs)) return -22;
@@ -287,12 +354,12 @@ extern "C" int hallo_rope(const hallo_rope_desc* d, void* stream) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) |
                          (uintptr_t)(2 * (a.x_rs | a.y_rs | a.hd | (d->batch > 1 ? a.x_bs | a.y_bs : 0)));
   // tokens of a workgroup: enough to fill its lanes and the cos / sin table, few enough to spread over the 256 CUs
-  // pieces of 4 columns: 150 us direct, 214 us staged (262144 tokens, 16 heads of 40); pieces of 1: 26 us direct, under 19 us staged (8510
+  // pieces of 4 columns: 150 us direct, 214 us staged (262144 tokens, 16 heads of 40); pieces of 1: 26 us direct, 18 us staged (8510
   // tokens, 16 heads of 80)
   const bool staged = V <= 2;
   int tt = ROPE_PAIRS / a.pairs;
   if (tt > ROPE_TT) tt = ROPE_TT;
-  if (staged && tt * a.hd > ROPE_STAGE) tt = ROPE_STAGE / a.hd;
+  if (staged && tt * width > ROPE_STAGE) tt = width <= ROPE_STAGE ? (int)(ROPE_STAGE / width) : 1;      // all heads of a token in one tile
   while (tt > 1 && (a.tokens + tt - 1) / tt < 1024) tt = (tt + 1) / 2;
   a.tt = tt;
   hipStream_t st = (hipStream_t)stream;

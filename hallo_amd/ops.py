@@ -998,6 +998,8 @@ def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
         out = torch.empty_like(x)
     else:
         _like("out", out, x)
+    if L >= 2 ** 31 - 64 or W // hd > 1 << 16:
+        _bad(f"x: at most 2^31 - 65 tokens of 2^16 heads, got {tuple(sh)}")
     so = out.stride()
     if so[2] != 1 or (L > 1 and so[1] < W) or (B > 1 and L and not so[0]):
         _bad(f"out: expected {tuple(sh)} with rows that do not overlap, got {tuple(out.shape)} strides {so}")

@@ -141,3 +141,19 @@ def test_nothing_to_do():
     axes = ops.RopeAxes((8,), 8)
     assert ops.rope(torch.empty(2, 0, 8, device="cuda", dtype=torch.float16), axes, pos=torch.empty(0, 1, device="cuda", dtype=torch.int32)).shape == (2, 0, 8)
     assert ops.rope(torch.empty(0, 3, 8, device="cuda", dtype=torch.float16), axes, grid=(3,)).shape == (0, 3, 8)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dims,hd", [((6, 10), 24), ((8, 16), 32), ((6, 8), 20)])
+def test_no_number_stays_where_it_is(dims, hd, interleaved):
+    """A NaN or an infinity reaches its pair, at every angle, and nothing else; columns that pass through keep theirs."""
+    from hallo_amd import ops
+    axes = ops.RopeAxes(dims, hd, interleaved=interleaved)
+    pos = torch.tensor([[0, 0], [3, 0], [0, 5]], device="cuda", dtype=torch.int32)
+    for bad in (float("nan"), float("inf")):
+        for col in range(hd):
+            x = torch.ones(1, 3, 2 * hd, device="cuda", dtype=torch.float16)
+            x[..., hd + col] = bad
+            got = torch.isfinite(ops.rope(x, axes, pos=pos))
+            want = torch.isfinite(_ref(x, dims, hd, pos[None], 10000.0, interleaved, False)[0])
+            assert torch.equal(got, want), (bad, col)
