@@ -2,13 +2,13 @@
 //
 //   P = exp(scale q k^T - lse) over the visible pairs,   delta = sum_d(do * o)
 //   dV = P^T dO,   dS = P * (dO V^T - delta),   dQ = scale dS K,   dK = scale dS^T Q
-// summed over the query heads that share a key head.  Three launches, four with split keys:
+// summed over the query heads that share a key head.  Three launches, and one for each kind of parts:
 //   prep   delta and lse * log2(e) of every query (fp32; +inf where a query has no visible key, so its P is 0)
 //   dkv    a workgroup owns 128 keys: K and V stay in registers as MFMA operands, dK and dV as accumulators, and the query rows that see
 //          the keys stream through LDS, for all heads of the group -- shared heads need no atomics
 //   dq     a workgroup owns 128 queries of a head (a wave 32), the visible keys stream through LDS
 //   join   the sinks are seen by every query: their key tiles' query rows are split over workgroups, fp32 parts are added here in order
-//          (also used for all keys when there are too few key tiles to fill the chip)
+//          (also used for all keys when there are too few key tiles to fill the chip, and for dq's keys when there are few queries)
 // S and dO V^T are computed in both dkv and dq (7 products where 5 would do with atomics on dQ): results do not depend on timing.
 //
 // fp16: P is 1/N over long rows and dS smaller still, below fp16's normal numbers.  Both are carried scaled by powers of two that cannot
@@ -35,6 +35,7 @@ struct WinBwdArgs {
   int nst, nrt, sps, spr;                        // key tiles of the sinks / of the rest, query splits of each
   float* part;                                   // [batch, kv_heads][nst * sps (if sps > 1) + nrt * spr (if spr > 1)][128][2 hd]
   int nparts;                                    // part tiles of one (batch entry, key head)
+  int spq; float* qpart;                         // key splits of dq, [batch, heads, Lq][spq][hd]
 };
 
 constexpr int BW_KEYS = 128;                     // keys of a dkv workgroup
@@ -400,7 +401,9 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
   win_lds* const lds = (win_lds*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, l31 = lane & 31;
-  int bid = xcd_remap(blockIdx.x, p.batch * p.heads * p.nqb);
+  int bid = xcd_remap(blockIdx.x, p.batch * p.heads * p.nqb * a.spq);
+  const int split = bid % a.spq;
+  bid /= a.spq;
   const int qb = p.nqb - 1 - bid % p.nqb;
   bid /= p.nqb;
   const int h = bid % p.heads, b = bid / p.heads, hk = h / p.group;
@@ -439,7 +442,8 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
 
   WinRange r = {0, 0, 0};
   if (i0 < qn) r = win_range(p, shift + i0, shift + min(i0 + 127, qn - 1), kn);
-  const int n0 = (r.e0 + KB - 1) / KB, nt = n0 + (r.e1 - r.s1 + KB - 1) / KB;
+  const int n0 = (r.e0 + KB - 1) / KB, all_t = n0 + (r.e1 - r.s1 + KB - 1) / KB;
+  const int tb = (int)((long)all_t * split / a.spq), nt = (int)((long)all_t * (split + 1) / a.spq);      // tiles tb .. nt - 1
   const int pw0 = shift + iw, pw1 = shift + min(iw + 31, qn - 1), pos = shift + row;
   const int vhi = p.right < 0 ? kn : min(kn, pos + p.right + 1), vlo = p.left < 0 ? 0 : pos - p.left;
 
@@ -493,11 +497,11 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
   const Tile tl(lane);
   const float c = p.c;
 
-  if (nt > 0) { load(0); store(0); }
+  if (nt > tb) { load(tb); store(tb & 1); }
   win_loads_done();
-  if (nt > 1) load(1);
+  if (nt > tb + 1) load(tb + 1);
   __syncthreads();
-  for (int t = 0; t < nt; ++t) {
+  for (int t = tb; t < nt; ++t) {
     const int j0 = t < n0 ? t * KB : r.s1 + (t - n0) * KB, end = t < n0 ? r.e0 : r.e1;
     if (t + 1 < nt) store((t + 1) & 1);
     if (t + 2 < nt) load(t + 2);
@@ -534,6 +538,19 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
     __syncthreads();
   }
   if (row >= p.Lq) return;
+  if (a.spq > 1) {
+    float* part = a.qpart + (at * a.spq + split) * p.hd;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = db * 32 + 8 * g + 4 * hi;
+        if (d < p.hd)
+          *reinterpret_cast<f32x4*>(part + d) = row < qn ? f32x4{dq[db][4 * g] * undo, dq[db][4 * g + 1] * undo, dq[db][4 * g + 2] * undo, dq[db][4 * g + 3] * undo}
+                                                        : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+    return;
+  }
   T* O = reinterpret_cast<T*>(a.dq) + (long)b * a.dq_bs + (long)h * a.dq_hs + (long)row * a.dq_rs;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
@@ -549,8 +566,30 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
     }
 }
 
-// Key tiles and query splits.  A sink tile meets every query, a tile of the rest at most left + right + 128 of them: the sinks' queries
-// are split so that their workgroups end with the others; and all are split when the tiles alone leave CUs idle.
+// dq of the query rows whose keys were split: 4 columns per thread, the parts are added in order
+template <typename T>
+__global__ __launch_bounds__(256) void win_bwd_join_q_kernel(const WinBwdArgs a) {
+  using V4 = typename Vec<T>::v4;
+  const WinArgs& p = a.w;
+  const int per = p.hd / 4;
+  const long k = (long)blockIdx.x * 256 + threadIdx.x, at = k / per;
+  const int d = (int)(k - at * per) * 4;
+  if (at >= (long)p.batch * p.heads * p.Lq) return;
+  const float* part = a.qpart + at * a.spq * p.hd + d;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < a.spq; ++i) s += *reinterpret_cast<const f32x4*>(part + (long)i * p.hd);
+  const long bh = at / p.Lq;
+  const int i = (int)(at - bh * p.Lq), h = (int)(bh % p.heads), b = (int)(bh / p.heads);
+  V4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(s[e]);
+  *reinterpret_cast<V4*>(reinterpret_cast<T*>(a.dq) + (long)b * a.dq_bs + (long)h * a.dq_hs + (long)i * a.dq_rs + d) = w;
+}
+
+// Key tiles and query splits.  A sink tile meets every query, a tile of the rest at most left + right + 128 of them, and there may be fewer
+// tiles than the chip takes at once: queries are split so that a workgroup has at most `target` steps of 32 query rows, the least
+// number of steps with which all workgroups run at once (two per CU up to 64 columns, else one).  Below 8 steps the parts cost more than
+// they save.
 int64_t plan_bwd(WinBwdArgs& a) {
   WinArgs& p = a.w;
   p.nqb = (p.Lq + 127) / 128;
@@ -560,16 +599,24 @@ int64_t plan_bwd(WinBwdArgs& a) {
   a.nrt = (p.Lk - s_end + BW_KEYS - 1) / BW_KEYS;
   a.nq64 = (p.Lq + 63) / 64;
   a.nk64 = (p.Lk + 63) / 64;
-  const long bh = (long)p.batch * p.kv_heads;
+  const long bh = (long)p.batch * p.kv_heads, slots = p.hd <= 64 ? 512 : 256;
   long span = p.Lq;
   if (p.left >= 0 && p.right >= 0 && (long)p.left + p.right + BW_KEYS < span) span = (long)p.left + p.right + BW_KEYS;
   const long it_s = (long)p.group * ((p.Lq + 31) / 32), it_r = (long)p.group * ((span + 31) / 32);
-  const auto fit = [](long want, long its) { const long m = its / 4; return (int)(want < 1 || m < 1 ? 1 : (want < m ? want : m)); };
-  a.spr = a.nrt && bh * a.nrt < 256 ? fit(512 / (bh * a.nrt), it_r) : 1;
-  long ws = it_r * 2 ? (it_s * a.spr + it_r - 1) / it_r : 1;
-  if (a.nst && bh * a.nst * ws < 256 && a.nrt * bh < 256) ws = 512 / (bh * a.nst);
-  if (ws > 64) ws = 64;
-  a.sps = a.nst ? fit(ws, it_s) : 1;
+  const auto parts = [](long its, long target) { const long n = (its + target - 1) / target; return n < 1 ? 1L : n; };
+  long target = 8;
+  while (target < it_r && bh * (a.nst * parts(it_s, target) + a.nrt * parts(it_r, target)) > slots) target += (target + 7) / 8;
+  if (target > it_r) target = it_r;              // more tiles than slots: only the sinks are split, into pieces as long as the others
+  if (target < 8) target = 8;
+  a.sps = a.nst ? (int)parts(it_s, target) : 1;
+  a.spr = a.nrt ? (int)parts(it_r, target) : 1;
+  // dq: few queries leave CUs idle, then the keys are split (two workgroups per CU, at least 8 tiles of 32 keys each)
+  long keys = p.Lk;
+  if (p.left >= 0 && p.right >= 0 && (long)p.left + p.right + p.Lq + p.sinks < keys) keys = (long)p.left + p.right + p.Lq + p.sinks;
+  const long blocks = (long)p.batch * p.heads * p.nqb, tiles = (keys + 31) / 32;
+  long sq = blocks > 0 && blocks < 256 ? 512 / blocks : 1;
+  if (sq > tiles / 8) sq = tiles / 8;
+  a.spq = sq < 1 ? 1 : (int)sq;
   a.nparts = (a.sps > 1 ? a.nst * a.sps : 0) + (a.spr > 1 ? a.nrt * a.spr : 0);
   const int64_t rows = (int64_t)p.batch * p.heads * p.Lq;
   int64_t at = 0;
@@ -580,6 +627,7 @@ int64_t plan_bwd(WinBwdArgs& a) {
   a.domax = base + take((int64_t)p.batch * p.heads * a.nq64);
   a.vmax = base + take(bh * a.nk64);
   a.part = base + take(bh * a.nparts * BW_KEYS * 2 * p.hd);
+  a.qpart = base + take(a.spq > 1 ? rows * a.spq * p.hd : 0);
   return at * 4;
 }
 
@@ -592,7 +640,7 @@ int launch_hk(const WinBwdArgs& a, hipStream_t st) {
     HALLO_CHECK_LAUNCH();
   }
   if (p.Lq > 0) {
-    hipLaunchKernelGGL((win_bwd_dq_kernel<T, HK>), dim3((unsigned)(p.batch * p.heads * p.nqb)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((win_bwd_dq_kernel<T, HK>), dim3((unsigned)(p.batch * p.heads * p.nqb * a.spq)), dim3(256), 0, st, a);
     HALLO_CHECK_LAUNCH();
   }
   return 0;
@@ -624,6 +672,11 @@ int launch(const WinBwdArgs& a, hipStream_t st) {
   const long nj = (long)p.batch * p.kv_heads * ((a.sps > 1 ? a.nst : 0) + (a.spr > 1 ? a.nrt : 0)) * 16;
   if (nj > 0) {
     hipLaunchKernelGGL((win_bwd_join_kernel<T>), dim3((unsigned)nj), dim3(256), 0, st, a);
+    HALLO_CHECK_LAUNCH();
+  }
+  if (a.spq > 1) {
+    const long n = (long)p.batch * p.heads * p.Lq * (p.hd / 4);
+    hipLaunchKernelGGL((win_bwd_join_q_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
     HALLO_CHECK_LAUNCH();
   }
   return 0;
