@@ -51,28 +51,31 @@ template <int HK> __device__ __forceinline__ int win_swz(int r) {
 template <int HK> struct WinTile {
   static constexpr int CH = HK / 8, PITCH = win_chunks(HK) * 16, NKS = HK / 16, NDB = (HK + 31) / 32;
   static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ win_swz<HK>(r)) << 4); }
-  // this lane's byte offsets: along[ks] of row (lane & 31), columns 16 ks + 8 hi; trans[db][k] of rows 8 k + .. read transposed
-  int along[NKS], trans[NDB][2];
+  // This lane's byte offsets: of row (lane & 31), columns 16 ks + 8 hi, and of rows 8 k + .. read transposed.  Where the swizzle stays
+  // within four chunks (32, 96, 160 columns) two of each serve all columns, the rest is part of the instruction.
+  static constexpr bool NEAR = win_chunks(HK) % 8 == 4;
+  static constexpr int NA = NEAR ? 2 : NKS, NB = NEAR ? 1 : NDB;
+  int along[NA], trans[NB][2];
   __device__ __forceinline__ WinTile(int lane) {
     const int hi = lane >> 5, l31 = lane & 31, gi = lane & 15, gdh = lane >> 4 & 1;
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) along[ks] = at(l31, ks * 2 + hi);
+    for (int ks = 0; ks < NA; ++ks) along[ks] = at(l31, ks * 2 + hi);
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
+    for (int db = 0; db < NB; ++db)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)                // columns past HK: operand rows whose products are not stored
-        trans[db][k] = at(8 * k + 4 * hi + (gi >> 2), min(db * 4 + gdh * 2, CH - 2) + (gi >> 1 & 1)) + (gi & 1) * 8;
+      for (int k = 0; k < 2; ++k)                // columns past HK (in the padding, or the last ones again): operand rows whose products are not stored
+        trans[db][k] = at(8 * k + 4 * hi + (gi >> 2), (NEAR ? gdh * 2 : min(db * 4 + gdh * 2, CH - 2)) + (gi >> 1 & 1)) + (gi & 1) * 8;
   }
   template <typename V8> __device__ __forceinline__ V8 row(const win_lds* tile, int row0, int ks) const {
-    return *(const __attribute__((address_space(3))) V8*)(tile + along[ks] + row0 * PITCH);
+    return *(const __attribute__((address_space(3))) V8*)(tile + (NEAR ? along[ks & 1] : along[ks % NA]) + row0 * PITCH + (NEAR ? (ks >> 1) * 64 : 0));
   }
   // Operand of a 32x32x16 MFMA whose 16-deep contraction runs over 16 LDS rows, read transposed: lane l holds column db * 32 + (l & 31)
   // of rows row0 + 4 hi + (e & 3) + 8 (e >> 2) (e = 0..7) -- the rows in which a 32x32 accumulator of the same wave holds its
   // registers, so a converted accumulator is the other operand as it stands.  row0: a multiple of 16
   template <typename V8> __device__ __forceinline__ V8 col(const win_lds* tile, int row0, int db) const {
     typedef __attribute__((address_space(3))) win_s16x4 lds4;
-    const win_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + trans[db][0] + row0 * PITCH));
-    const win_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + trans[db][1] + row0 * PITCH));
+    const win_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + trans[NEAR ? 0 : db][0] + row0 * PITCH + (NEAR ? db * 64 : 0)));
+    const win_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + trans[NEAR ? 0 : db][1] + row0 * PITCH + (NEAR ? db * 64 : 0)));
     return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };

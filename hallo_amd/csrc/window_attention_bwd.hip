@@ -396,6 +396,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
   using Tile = WinTile<HK>;
   constexpr int TB = KB * Tile::PITCH, STAGE = 2 * TB;   // K | V
   constexpr int U = (KB * CH + 255) / 256;
+  constexpr int AHEAD = HK > 128 || HK < 32 ? 2 : 4;     // LDS reads ahead of their MFMAs; 160 columns are at the register limit
   const WinArgs& p = a.w;
   __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
   win_lds* const lds = (win_lds*)smem;
@@ -515,7 +516,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
         s = Vec<T>::mfma32(tl.template row<V8>(kt, 0, ks), qf[ks], s);
         dp = Vec<T>::mfma32(tl.template row<V8>(vt, 0, ks), gf[ks], dp);
       }
-      win_order<2 * NKS, 1, NKS < 4 ? NKS : 4>();
+      win_order<2 * NKS, 1, AHEAD>();
       const bool all = end - j0 >= KB && (p.right < 0 || j0 + KB - 1 <= pw0 + p.right) &&
                        (p.left < 0 || j0 >= pw1 - p.left || j0 + KB <= p.sinks);
       const int lhi = min(vhi, end);
@@ -533,7 +534,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int h2 = 0; h2 < 2; ++h2) dq[db] = Vec<T>::mfma32(tl.template col<V8>(kt, h2 * 16, db), df[h2], dq[db]);
-      win_order<NDB * 2, 2, NDB * 2 < 4 ? 2 : 4>();
+      win_order<NDB * 2, 2, (AHEAD < NDB * 2 ? AHEAD : NDB * 2)>();
     }
     __syncthreads();
   }
