@@ -38,23 +38,22 @@ __device__ __forceinline__ WinRange win_range(const WinArgs& p, int plo, int phi
   return lo <= se ? WinRange{hi, hi, hi} : WinRange{se, lo, hi};
 }
 
-// LDS tiles of rows of HK elements (a multiple of 16): rows of win_chunks(HK) 16-byte chunks, chunk c of row r stored at c ^ win_swz(r).
-// A tile is read along its rows (MFMA operand, 16 bytes per lane, lane = row: 16 consecutive rows at one chunk) and transposed (32
-// lanes: 4 consecutive rows x 64 aligned bytes); the swizzle puts both kinds of 256 bytes on all 64 banks once.  It repeats every 16
-// rows, so a fragment further down the tile is an immediate offset away.  (Padded pitches without a swizzle serve one kind only: a
-// quarter of the forward kernel's LDS cycles were conflicts.)
-constexpr int win_chunks(int HK) { return HK == 48 ? 8 : HK == 80 ? 12 : HK == 112 ? 16 : HK == 144 ? 20 : HK / 8; }
-template <int HK> __device__ __forceinline__ int win_swz(int r) {
-  constexpr int C = win_chunks(HK);
-  return C == 16 ? (r & 3) << 2 | (r >> 2 & 3) : C == 8 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : C == 2 ? r >> 3 & 1 : r >> 2 & 3;
-}
-template <int HK> struct WinTile {
-  static constexpr int CH = HK / 8, PITCH = win_chunks(HK) * 16, NKS = HK / 16, NDB = (HK + 31) / 32;
-  static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ win_swz<HK>(r)) << 4); }
-  // This lane's byte offsets: of row (lane & 31), columns 16 ks + 8 hi, and of rows 8 k + .. read transposed.  Where the swizzle stays
-  // within four chunks (32, 96, 160 columns) two of each serve all columns, the rest is part of the instruction.
-  static constexpr bool NEAR = win_chunks(HK) % 8 == 4;
+// LDS tiles of rows of HK elements (a multiple of 16): rows of C 16-byte chunks, chunk c of row r stored at c ^ swz(r).  A tile is read
+// along its rows (MFMA operand, 16 bytes per lane, lane = row: 16 consecutive rows at one chunk) and transposed (32 lanes: 4 consecutive
+// rows x 64 aligned bytes); the swizzle puts both kinds of 256 bytes on all 64 banks once.  It repeats every 16 rows, so a fragment
+// further down the tile is an immediate offset away.  (Padded pitches without a swizzle serve one kind only: a quarter of the forward
+// kernel's LDS cycles were conflicts.)
+// C = 4, 12 or 20: consecutive rows start four chunks apart (mod 16) and the swizzle stays within four chunks, so two lane offsets of
+// each kind serve all columns and the rest is part of the instruction.  C = 16 is denser, for the kernel that is short of LDS.
+constexpr int win_chunks(int HK) { return HK <= 32 ? 4 : HK <= 96 ? 12 : 20; }
+template <int HK, int C = win_chunks(HK)> struct WinTile {
+  static_assert(C * 8 >= HK && (C % 8 == 4 || C == 16), "");
+  static constexpr bool NEAR = C % 8 == 4;
+  static constexpr int PITCH = C * 16, NKS = HK / 16, NDB = (HK + 31) / 32;
   static constexpr int NA = NEAR ? 2 : NKS, NB = NEAR ? 1 : NDB;
+  static __device__ __forceinline__ int swz(int r) { return NEAR ? r >> 2 & 3 : (r & 3) << 2 | (r >> 2 & 3); }
+  static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ swz(r)) << 4); }
+  // this lane's byte offsets: of row (lane & 31), columns 16 ks + 8 hi, and of rows 8 k + .. read transposed
   int along[NA], trans[NB][2];
   __device__ __forceinline__ WinTile(int lane) {
     const int hi = lane >> 5, l31 = lane & 31, gi = lane & 15, gdh = lane >> 4 & 1;
@@ -63,11 +62,11 @@ template <int HK> struct WinTile {
 #pragma unroll
     for (int db = 0; db < NB; ++db)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)                // columns past HK (in the padding, or the last ones again): operand rows whose products are not stored
-        trans[db][k] = at(8 * k + 4 * hi + (gi >> 2), (NEAR ? gdh * 2 : min(db * 4 + gdh * 2, CH - 2)) + (gi >> 1 & 1)) + (gi & 1) * 8;
+      for (int k = 0; k < 2; ++k)                // columns past HK lie in the padding: operand rows whose products are not stored
+        trans[db][k] = at(8 * k + 4 * hi + (gi >> 2), db * 4 + gdh * 2 + (gi >> 1 & 1)) + (gi & 1) * 8;
   }
   template <typename V8> __device__ __forceinline__ V8 row(const win_lds* tile, int row0, int ks) const {
-    return *(const __attribute__((address_space(3))) V8*)(tile + (NEAR ? along[ks & 1] : along[ks % NA]) + row0 * PITCH + (NEAR ? (ks >> 1) * 64 : 0));
+    return *(const __attribute__((address_space(3))) V8*)(tile + along[ks % NA] + row0 * PITCH + (NEAR ? (ks >> 1) * 64 : 0));
   }
   // Operand of a 32x32x16 MFMA whose 16-deep contraction runs over 16 LDS rows, read transposed: lane l holds column db * 32 + (l & 31)
   // of rows row0 + 4 hi + (e & 3) + 8 (e >> 2) (e = 0..7) -- the rows in which a 32x32 accumulator of the same wave holds its

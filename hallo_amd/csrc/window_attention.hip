@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   using V8 = typename Vec<T>::v8;
   constexpr int NKS = HK / 16, NDB = (HK + 31) / 32, OP = HK + 4;      // OP: pitch of the joined rows, floats
   constexpr float NEG_INF = -__builtin_inff();
-  using Tile = WinTile<HK>;
+  using Tile = WinTile<HK, HK == 112 || HK == 128 ? 16 : win_chunks(HK)>;      // eight tiles of a workgroup: two workgroups per CU at 128 columns
   constexpr int TB = 32 * Tile::PITCH, WT = 4 * 2 * TB, JT = 32 * OP * 4;      // LDS: K | V of every wave, then the joined rows
   __shared__ __attribute__((aligned(16))) unsigned char smem[WT > JT ? WT : JT];
   __shared__ float sm_m[4][32], sm_l[4][32];
