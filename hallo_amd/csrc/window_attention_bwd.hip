@@ -41,6 +41,11 @@ struct WinBwdArgs {
 constexpr int BW_KEYS = 128;                     // keys of a dkv workgroup
 constexpr float P_EXP = 14.0f;                   // fp16: P is carried times 2^14
 
+// whether some query of the entry sees key j < kn (the queries stand at shift .. kn - 1); what lies elsewhere may hold anything
+__device__ __forceinline__ bool key_seen(const WinArgs& p, int j, int shift, int qn) {
+  return qn > 0 && (p.left < 0 || j < p.sinks || shift - p.left <= j);
+}
+
 // 2^e with 2 a b 2^e < 2^15
 __device__ __forceinline__ float ds_scale(float a, float b) {
   const float bound = 2.0f * a * b;
@@ -61,7 +66,7 @@ __global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, i
   const int nb = isq ? a.nq64 : a.nk64, heads = isq ? p.heads : p.kv_heads;
   const int blk = bid % nb; bid /= nb;
   const int h = bid % heads, b = bid / heads;
-  const int n = isq ? win_len(p.q_len, b, p.Lq) : win_len(p.kv_len, b, p.Lk);
+  const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk), n = isq ? qn : kn;
   float big = 0.0f;
   V8 xv[4][2], ov[4][2];                         // 16 lanes share a row, a lane's columns are 8 sub and 128 + 8 sub; four rows in flight
 #pragma unroll
@@ -73,7 +78,7 @@ __global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, i
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int d = sub * 8 + 128 * c;
-      const bool ok = i < n && d < p.hd;
+      const bool ok = i < n && d < p.hd && (isq || key_seen(p, i, kn - qn, qn));
       xv[k][c] = ok ? ld8<T>(x + d) : zero8<T>();
       ov[k][c] = ok && isq ? ld8<T>(o + d) : zero8<T>();
     }
@@ -166,12 +171,13 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
                     : reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hk * p.k_hs;
   const long w_rs = role ? p.v_rs : p.k_rs;
   const int kw = ka + kg * 32, key = kw + l31;
+  const bool seen = key < kb && key_seen(p, key, shift, qn);
   V8 wf[NKS];                                    // this lane's key row of K (role 0) or V (role 1)
   float wsq = 0.0f;
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) {
     const int d = ks * 16 + hi * 8;
-    wf[ks] = key < kb && d < p.hd ? ld8<T>(W + (long)key * w_rs + d) : zero8<T>();
+    wf[ks] = seen && d < p.hd ? ld8<T>(W + (long)key * w_rs + d) : zero8<T>();
     if (F16)
 #pragma unroll
       for (int e = 0; e < 8; ++e) { const float f = to_f32(wf[ks][e]); wsq += f * f; }

@@ -1041,8 +1041,13 @@ def _heads4(name, t, heads, hd, writable=False):
         bs, rs, hs = st[:3] if ok else (0, 0, 0)
     if not ok:
         _bad(f"{name}: expected [B, L, {heads} * {hd}] or [B, L, {heads}, {hd}] with contiguous heads, got {tuple(sh)} strides {st}")
-    if writable and ((sh[0] > 1 and not bs) or (sh[1] > 1 and not rs) or (heads > 1 and not hs)):
-        _bad(f"{name}: overlapping rows, strides {st}")
+    if writable:
+        extent = hd
+        for s, n in sorted(((bs, sh[0]), (rs, sh[1]), (hs, heads))):
+            if n > 1:
+                if s < extent:
+                    _bad(f"{name}: overlapping rows, strides {st}")
+                extent += (n - 1) * s
     # strides of single or absent rows, entries and heads never count
     if sh[0] <= 1:
         bs = 0
@@ -1059,7 +1064,7 @@ def _edge(n):
     return -1 if n < 0 else min(int(n), 1 << 29)
 
 
-def _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, o_written):
+def _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, o_given):
     """(descriptor without workspace, kv_heads, head_dim) of checked arguments."""
     code = dtype_code(q.dtype)
     if kv_heads is None:
@@ -1094,7 +1099,7 @@ def _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv
         _bad(f"scale: expected a positive number, got {scale}")
     d = _l.WindowAttnDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None,
                           *_heads4("q", q, heads, hd), *_heads4("k", k, kv_heads, hd), *_heads4("v", v, kv_heads, hd),
-                          *_heads4("out" if o_written else "o", o, heads, hd, o_written),
+                          *_heads4("out" if o_given else "o", o, heads, hd, o_given),
                           q_len.data_ptr() if q_len is not None else None, kv_len.data_ptr() if kv_len is not None else None,
                           Lq, Lk, B, heads, kv_heads, hd, _edge(left), _edge(right), _edge(sinks), scale, code)
     return d, kv_heads, hd
@@ -1113,12 +1118,13 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
 
     return_lse: (out, lse), lse fp32 [B, heads, Lq] (-inf where nothing is visible), as window_attention_backward() takes it."""
     _chk_dev(q, k, v, q_len, kv_len, out)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(q)
     else:
         _like("out", out, q)
     lse = torch.empty((q.shape[0], heads, q.shape[1]), device=q.device, dtype=torch.float32) if return_lse and heads >= 1 else None
-    d, _, _ = _window_desc(q, k, v, out, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, True)
+    d, _, _ = _window_desc(q, k, v, out, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, given)
     need = _l.load().hallo_window_attention_workspace(C.byref(d))
     if need:
         if need < 0:
@@ -1140,16 +1146,17 @@ def window_attention_backward(do, q, k, v, o, lse, heads, *, kv_heads=None, left
     if lse.shape != (q.shape[0], heads, q.shape[1]) or not lse.is_contiguous():
         _bad(f"lse: expected contiguous ({q.shape[0]}, {heads}, {q.shape[1]}), got {tuple(lse.shape)}")
     w, kv_heads, hd = _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, False)
-    outs = []
-    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        if t is None:
-            t = torch.empty(like.shape, device=q.device, dtype=q.dtype)
-        else:
+    outs, strides = [], []
+    for name, t, like, n in (("dq", dq, q, heads), ("dk", dk, k, kv_heads), ("dv", dv, v, kv_heads)):
+        given = t is not None
+        if given:
             _like(name, t, like)
+        else:
+            t = torch.empty(like.shape, device=q.device, dtype=q.dtype)
         outs.append(t)
+        strides += _heads4(name, t, n, hd, given)
     dq, dk, dv = outs
-    d = _l.WindowAttnBwdDesc(w, do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *_heads4("do", do, heads, hd),
-                             *_heads4("dq", dq, heads, hd, True), *_heads4("dk", dk, kv_heads, hd, True), *_heads4("dv", dv, kv_heads, hd, True))
+    d = _l.WindowAttnBwdDesc(w, do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *_heads4("do", do, heads, hd), *strides)
     need = _l.load().hallo_window_attention_backward_workspace(C.byref(d))
     if need < 0:
         _l.check(need, "hallo_window_attention_backward_workspace")

@@ -251,6 +251,8 @@ def test_window_attention_arguments(host):
     r(q, torch.zeros(2, 32, 7, dtype=h).transpose(1, 2), k, 4, match="contiguous")
     r(q, k, k, 4, out=q[:, :4], match="out")
     r(q, k, k, 4, out=q[:1].expand(2, -1, -1), match="overlap")
+    r(q, k, k, 4, out=torch.zeros(1000, dtype=h).as_strided((2, 5, 64), (320, 56, 1)), match="overlap")
+    r(q.view(2, 5, 4, 16), k, k, 4, out=torch.zeros(1000, dtype=h).as_strided((2, 5, 4, 16), (320, 64, 8, 1)), match="overlap")
     lse = torch.zeros(2, 4, 5)
 
     def b(*a, match=None, **kw):

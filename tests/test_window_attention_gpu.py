@@ -226,6 +226,26 @@ def test_hidden_keys_between(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+def test_hidden_keys_in_the_backward_pass(dtype):
+    """Queries at the end of the keys with a window: keys that no query sees hold garbage; their gradients are zeros and the others do
+    not know of them (large finite values would take the fp16 scale down, infinities take it away)."""
+    from hallo_amd import ops
+    for Lq, left, sinks in ((5, 63, 3), (100, 20, 0), (1, 0, 1)):
+        q, k, v, do = _qkv(2, Lq, 400, 4, 2, 64, dtype, Lq)
+        ql, kl = _lens(Lq, max(1, Lq - 2)), _lens(400, 333)
+        kw = dict(kv_heads=2, left=left, sinks=sinks, q_len=ql, kv_len=kl)
+        ref = Ref(q, k, v, 4, 2, left, 0, sinks, ql, kl)
+        o, lse = ops.window_attention(q, k, v, 4, return_lse=True, **kw)
+        clean = ops.window_attention_backward(do, q, k, v, o, lse, 4, **kw)
+        ref.check_grads(do, o, lse, *clean)
+        gone = ~ref.ok.any(2).reshape(2, 400)
+        for bad in (float("nan"), float("inf"), 30000.0):
+            k[gone], v[gone] = bad, -bad
+            got = ops.window_attention_backward(do, q, k, v, o, lse, 4, **kw)
+            assert all(torch.equal(a, b) for a, b in zip(got, clean))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("H,Hkv", [(1, 1), (7, 1), (8, 8), (12, 4), (32, 2)])
 def test_single_tokens_follow_the_prompt(dtype, H, Hkv):
     """A cache filled token by token answers as the whole sequence does."""
