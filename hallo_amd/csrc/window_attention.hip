@@ -396,12 +396,15 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
     p.lse[((long)b * p.heads + h) * p.Lq + ir] = Lr > 0.0f ? (Mr * c + __builtin_amdgcn_logf(Lr)) * 0.69314718055994530942f : (inv != 0.0f ? inv : NEG_INF);
 }
 
-// one wave per query row: joins the parts of its key splits
+// one wave per query row: joins the parts of its key splits.  The splits' shares are computed side by side by the lanes, so that the loop
+// over the parts is loads that do not wait for one another.
+constexpr int WIN_MAX_SPLIT = 512;
 template <typename T>
 __global__ __launch_bounds__(256) void win_join_kernel(const WinArgs p) {
-  const int lane = threadIdx.x & 63;
+  __shared__ float share[4][WIN_MAX_SPLIT];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int rows = p.group * p.Lq;
-  const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long id = (long)blockIdx.x * 4 + wave;
   if (id >= (long)p.batch * p.kv_heads * rows) return;
   const int R = (int)(id % rows);
   const long bh = id / rows;
@@ -411,14 +414,20 @@ __global__ __launch_bounds__(256) void win_join_kernel(const WinArgs p) {
   float M = -__builtin_inff();
   for (int s = lane; s < p.nsplit; s += 64) M = fmaxf(M, part[(long)s * step]);
   M = wave_max(M);
-  float L = 0.0f, acc[3] = {0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float* q = part + (long)s * step;
-    const float f = q[0] == M ? 1.0f : __builtin_amdgcn_exp2f((q[0] - M) * p.c);
-    L += q[1] * f;
+  float L = 0.0f;
+  for (int s = lane; s < p.nsplit; s += 64) {
+    const float m = part[(long)s * step], f = m == M ? 1.0f : __builtin_amdgcn_exp2f((m - M) * p.c);
+    share[wave][s] = f;
+    L += part[(long)s * step + 1] * f;
+  }
+  L = wave_sum(L);
+  float acc[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int s = 0; s < p.nsplit; ++s) {           // share: written and read by this wave alone
+    const float f = share[wave][s];
+    const float* q = part + (long)s * step + 2;
 #pragma unroll
-    for (int k = 0; k < 3; ++k)
-      if (lane + 64 * k < p.hd) acc[k] += q[2 + lane + 64 * k] * f;
+    for (int k = 0; k < 3; ++k) acc[k] += (lane + 64 * k < p.hd ? q[lane + 64 * k] : 0.0f) * f;
   }
   const int gr = R / p.Lq, i = R - gr * p.Lq, h = hk * p.group + gr;
   const float inv = L > 0.0f ? 1.0f / L : (L != L ? L : 0.0f);
@@ -443,6 +452,10 @@ void plan(WinArgs& a) {
   const long wgs = (long)a.batch * a.kv_heads * a.nrb, tiles = (keys + 31) / 32;
   long ns = (512 + wgs - 1) / wgs;
   if (ns > tiles / 4) ns = tiles / 4;            // every wave of a split has a tile
+  // the second launch and the parts cost what the split saves: one stream of 12 heads of 64 takes 11.4 us against 1024 keys in one piece
+  // and in eight, 8.3 and 10.1 us against 512
+  if (tiles * a.hd <= 2560) ns = 1;
+  if (ns > WIN_MAX_SPLIT) ns = WIN_MAX_SPLIT;
   a.nsplit = ns < 1 ? 1 : (int)ns;
 }
 

@@ -54,7 +54,7 @@ __device__ __forceinline__ float ds_scale(float a, float b) {
   return __builtin_amdgcn_ldexpf(1.0f, min(e, 110));
 }
 
-template <typename T>
+template <typename T, int NC>
 __global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, int qblocks) {
   using V8 = typename Vec<T>::v8;
   constexpr bool F16 = std::is_same<T, _Float16>::value;
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, i
   const int h = bid % heads, b = bid / heads;
   const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk), n = isq ? qn : kn;
   float big = 0.0f;
-  V8 xv[4][2], ov[4][2];                         // 16 lanes share a row, a lane's columns are 8 sub and 128 + 8 sub; four rows in flight
+  V8 xv[4][NC], ov[4][NC];                       // 16 lanes share a row, a lane's columns start at 8 sub (and 128 + 8 sub); four rows in flight
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int i = blk * 64 + k * 16 + grp;
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, i
                      : reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)h * p.v_hs + (long)i * p.v_rs;
     const T* o = reinterpret_cast<const T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)i * p.o_rs;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < NC; ++c) {
       const int d = sub * 8 + 128 * c;
       const bool ok = i < n && d < p.hd && (isq || key_seen(p, i, kn - qn, qn));
       xv[k][c] = ok ? ld8<T>(x + d) : zero8<T>();
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void win_bwd_prep_kernel(const WinBwdArgs a, i
     const int i = blk * 64 + k * 16 + grp;
     float dl = 0.0f, sq = 0.0f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float f = to_f32(xv[k][c][e]);
@@ -387,6 +387,7 @@ __global__ __launch_bounds__(256) void win_bwd_join_kernel(const WinBwdArgs a) {
     const int kl = rows8 * 8 + k / w, d = k % w, j = ka + kl;
     if (j >= kz) continue;
     float s = 0.0f;
+#pragma unroll 8
     for (int i = 0; i < sp; ++i) s += part[(long)i * BW_KEYS * w + (long)kl * w + d];
     if (d < p.hd) dK[(long)j * a.dk_rs + d] = from_f32<T>(s);
     else dV[(long)j * a.dv_rs + d - p.hd] = from_f32<T>(s);
@@ -584,6 +585,7 @@ __global__ __launch_bounds__(256) void win_bwd_join_q_kernel(const WinBwdArgs a)
   if (at >= (long)p.batch * p.heads * p.Lq) return;
   const float* part = a.qpart + at * a.spq * p.hd + d;
   f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
   for (int i = 0; i < a.spq; ++i) s += *reinterpret_cast<const f32x4*>(part + (long)i * p.hd);
   const long bh = at / p.Lq;
   const int i = (int)(at - bh * p.Lq), h = (int)(bh % p.heads), b = (int)(bh / p.heads);
@@ -659,7 +661,8 @@ int launch(const WinBwdArgs& a, hipStream_t st) {
   const bool f16 = std::is_same<T, _Float16>::value;
   const long qblocks = (long)p.batch * p.heads * a.nq64, kblocks = f16 ? (long)p.batch * p.kv_heads * a.nk64 : 0;
   if (qblocks + kblocks > 0) {
-    hipLaunchKernelGGL((win_bwd_prep_kernel<T>), dim3((unsigned)(qblocks + kblocks)), dim3(256), 0, st, a, (int)qblocks);
+    if (p.hd <= 128) hipLaunchKernelGGL((win_bwd_prep_kernel<T, 1>), dim3((unsigned)(qblocks + kblocks)), dim3(256), 0, st, a, (int)qblocks);
+    else hipLaunchKernelGGL((win_bwd_prep_kernel<T, 2>), dim3((unsigned)(qblocks + kblocks)), dim3(256), 0, st, a, (int)qblocks);
     HALLO_CHECK_LAUNCH();
   }
   int rc;
