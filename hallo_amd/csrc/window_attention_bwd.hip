@@ -12,9 +12,9 @@
 // S and dO V^T are computed in both dkv and dq (7 products where 5 would do with atomics on dQ): results do not depend on timing.
 //
 // fp16: P is 1/N over long rows and dS smaller still, below fp16's normal numbers.  Both are carried scaled by powers of two that cannot
-// overflow and are taken out of the fp32 accumulators at the end: P by 2^14 (P <= 1), dS by 2^e with |dS| <= 2 |do_i|_2 |v_j|_2 <
-// 2^(15 - e) -- in dkv the norm of the lane's own key row and the largest |do_i|, in dq the norm of the lane's own do row and the
-// largest |v_j|.  bf16 has fp32's range and needs neither.
+// overflow and are taken out of the fp32 accumulators at the end: P by 2^14 (P <= 1), dS by 2^e with |dS| = P |do_i . (v_j - o_i)| <=
+// 2 |do_i|_2 max_j |v_j|_2 < 2^(15 - e) -- in dkv with the largest |do_i| of the group, in dq with the lane's own do row.  (A key's own
+// |v_j| bounds nothing: o_i is as long as the longest v.)  bf16 has fp32's range and needs neither.
 #include <type_traits>
 #include "window_args.h"
 #include "../../include/hallo_amd.h"
@@ -141,7 +141,6 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
   constexpr int U = (QB * CH + 511) / 512;
   const WinArgs& p = a.w;
   __shared__ __attribute__((aligned(16))) unsigned char smem[3 * STAGE + 2 * 4 * PX];
-  __shared__ float sm_g[BW_KEYS];
   win_lds* const lds = (win_lds*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, l31 = lane & 31, kg = wave & 3;
@@ -173,25 +172,21 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
   const int kw = ka + kg * 32, key = kw + l31;
   const bool seen = key < kb && key_seen(p, key, shift, qn);
   V8 wf[NKS];                                    // this lane's key row of K (role 0) or V (role 1)
-  float wsq = 0.0f;
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) {
     const int d = ks * 16 + hi * 8;
     wf[ks] = seen && d < p.hd ? ld8<T>(W + (long)key * w_rs + d) : zero8<T>();
-    if (F16)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { const float f = to_f32(wf[ks][e]); wsq += f * f; }
   }
-  float gs = 1.0f;                               // fp16: scale of dS (relative to P's) for this lane's key
+  float g = 1.0f;                                // fp16: scale of dS
   if (F16 && role) {
-    float dm = 0.0f;
+    float dm = 0.0f, vm = 0.0f;
     const float* m = a.domax + ((long)b * p.heads + hk * p.group) * a.nq64;
+    const float* n = a.vmax + ((long)b * p.kv_heads + hk) * a.nk64;
     for (int i = lane; i < p.group * a.nq64; i += 64) dm = fmaxf(dm, m[i]);
-    dm = wave_max(dm);
-    const float g = ds_scale(dm, sqrtf(win_half_sum(wsq)));
-    if (hi == 0) sm_g[kg * 32 + l31] = 1.0f / g;
-    gs = g * 0x1p-14f;
+    for (int i = lane; i < a.nk64; i += 64) vm = fmaxf(vm, n[i]);
+    g = ds_scale(wave_max(dm), wave_max(vm));
   }
+  const float gs = g * 0x1p-14f;                 // relative to P's
 
   // positions that see this lane's key / that all of the group's keys are seen from / that see any of them
   constexpr int FAR = WIN_MAX_LEN * 2 - 1;
@@ -357,7 +352,7 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int kl = kg * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi, j = ka + kl;
-      const float f = role ? (F16 ? sm_g[kl] * p.scale : HALF_P ? p.scale * 0x1p-14f : p.scale) : (SCALED ? 0x1p-14f : 1.0f);
+      const float f = role ? (F16 ? p.scale / g : HALF_P ? p.scale * 0x1p-14f : p.scale) : (SCALED ? 0x1p-14f : 1.0f);
       const float v = j < kb ? acc[db][e] * f : 0.0f;
       if (part) part[(long)kl * 2 * p.hd + d] = v;
       else if (j < kz) D[(long)j * d_rs + d] = from_f32<T>(v);

@@ -246,6 +246,24 @@ def test_hidden_keys_in_the_backward_pass(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("small", [0.0, 2.0 ** -10, 2.0 ** -5])
+def test_small_values_under_large_probabilities(dtype, small):
+    """First keys that every query looks at and whose values are next to nothing: dS = P (dP - delta) is as large as the other keys'
+    values make delta, not as their own values make dP."""
+    from hallo_amd import ops
+    for B, L, H, Hkv, hd in ((1, 200, 4, 2, 64), (2, 300, 2, 2, 80), (16, 140, 8, 4, 40)):
+        q, k, v, do = _qkv(B, L, L, H, Hkv, hd, dtype, 5)
+        k[:, :2] = q[:, L // 2:L // 2 + 2].view(B, 2, Hkv, H // Hkv, hd)[:, :, :, 0].reshape(B, 2, Hkv * hd)
+        v[:, :2] *= small
+        v[:, 2:] *= 8.0
+        kw = dict(kv_heads=Hkv, left=50, sinks=4)
+        ref = Ref(q, k, v, H, Hkv, 50, 0, 4)
+        o, lse = ops.window_attention(q, k, v, H, return_lse=True, **kw)
+        ref.check(o, lse)
+        ref.check_grads(do, o, lse, *ops.window_attention_backward(do, q, k, v, o, lse, H, **kw))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("H,Hkv", [(1, 1), (7, 1), (8, 8), (12, 4), (32, 2)])
 def test_single_tokens_follow_the_prompt(dtype, H, Hkv):
     """A cache filled token by token answers as the whole sequence does."""
