@@ -498,7 +498,7 @@ int launch(const WinArgs& a, hipStream_t st) {
 bool win_args(const hallo_window_attn_desc* d, WinArgs& a) {
   if (!d || (d->dtype != DT_F16 && d->dtype != DT_BF16) || d->batch < 0 || d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads ||
       d->head_dim < 8 || d->head_dim > WIN_MAX_HD || d->head_dim % 8 || d->Lq < 0 || d->Lk < 0 || d->Lq > WIN_MAX_LEN || d->Lk > WIN_MAX_LEN ||
-      d->sinks < 0 || !(d->scale > 0.0f) || !(d->scale < 1e30f))
+      d->sinks < 0 || !(d->scale >= 1e-30f) || !(d->scale < 1e30f))
     return false;
   const int64_t strides[] = {d->q_bs, d->q_rs, d->q_hs, d->k_bs, d->k_rs, d->k_hs, d->v_bs, d->v_rs, d->v_hs, d->o_bs, d->o_rs, d->o_hs};
   for (int64_t s : strides)
@@ -509,7 +509,7 @@ bool win_args(const hallo_window_attn_desc* d, WinArgs& a) {
   const void* ptrs[] = {d->q, d->k, d->v, d->o};
   for (const void* p : ptrs)
     if (reinterpret_cast<uintptr_t>(p) & 15) return false;
-  if ((int64_t)d->batch * d->heads * ((d->Lq + 31) / 32) > 0x7fffffff || (int64_t)d->heads * d->Lq > 0x7fffffff ||
+  if ((int64_t)d->batch * d->heads * ((d->Lq + 31) / 32) > 0x7fffffff || (int64_t)d->heads * d->Lq > 0x7fffff00 ||
       (int64_t)d->batch * d->heads * ((d->Lk + 31) / 32) > 0x7fffffff)
     return false;
   const auto cut = [](int x) { return x > WIN_MAX_LEN ? WIN_MAX_LEN : x; };

@@ -1095,8 +1095,8 @@ def _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv
     if sinks < 0:
         _bad(f"sinks: {sinks}")
     scale = hd ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        _bad(f"scale: expected a positive number, got {scale}")
+    if not 1e-30 <= scale < 1e30:
+        _bad(f"scale: expected a positive number (1e-30 to 1e30), got {scale}")
     d = _l.WindowAttnDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None,
                           *_heads4("q", q, heads, hd), *_heads4("k", k, kv_heads, hd), *_heads4("v", v, kv_heads, hd),
                           *_heads4("out" if o_given else "o", o, heads, hd, o_given),

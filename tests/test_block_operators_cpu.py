@@ -137,6 +137,14 @@ def test_window_attention_abi(lib):
     assert lib.hallo_window_attention_workspace(C.byref(_attn_desc(p, Lq=1, Lk=100000, left=5, sinks=1))) == 0
 
 
+@pytest.mark.parametrize("kw", [dict(scale=1e-31), dict(heads=1 << 28, kv_heads=1 << 28, Lq=8)])
+def test_window_attention_limits(lib, kw):
+    """A scale whose rescaling threshold would overflow, query rows that pass 32 bits."""
+    keep, p = _mem()
+    assert lib.hallo_window_attention(C.byref(_attn_desc(p, **kw)), None) == -22
+    assert lib.hallo_window_attention_workspace(C.byref(_attn_desc(p, **kw))) == -22
+
+
 def test_window_attention_backward_abi(lib):
     keep, p = _mem()
 
