@@ -141,6 +141,11 @@ __device__ __forceinline__ float sum8_dpp(float v) {
   return v;
 }
 
+// between LDS accesses of different lanes of one wave: the hardware keeps their order, the compiler sees one lane and has to be told
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_join_kernel(const float* __restri
 #pragma unroll
   for (int k = 0; k < 16; ++k) t += sm[grp * 16 + k][cl];
   sm[grp * 16][cl] = t;                          // row grp * 16 is read by this thread alone
-  __builtin_amdgcn_wave_barrier();               // the four groups are one wave
+  wave_lds_order();                              // the four groups are one wave
   if (grp == 0 && c < 2 * C) {
     t = (sm[0][cl] + sm[16][cl]) + (sm[32][cl] + sm[48][cl]);
     if (c < C) dgamma[c] = t; else dbeta[c - C] = t;

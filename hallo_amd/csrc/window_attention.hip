@@ -302,6 +302,7 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
       *(__attribute__((address_space(3))) V8*)(kt + Tile::at(rr, ch)) = kr[i];
       *(__attribute__((address_space(3))) V8*)(vt + Tile::at(rr, ch)) = vr[i];
     }
+    wave_lds_order();
     if (t + 4 < te) load(t + 4);
     f32x16 s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
@@ -342,6 +343,7 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int h2 = 0; h2 < 2; ++h2) o[db] = Vec<T>::mfma32(tl.template col<V8>(vt, h2 * 16, db), pf[h2], o[db]);
+    wave_lds_order();
   }
   l = win_half_sum(l);
   if (!live) { m = NEG_INF; l = 0.0f; }          // rows without a query went along in the tiles that need no mask
@@ -421,9 +423,10 @@ __global__ __launch_bounds__(256) void win_join_kernel(const WinArgs p) {
     L += part[(long)s * step + 1] * f;
   }
   L = wave_sum(L);
+  wave_lds_order();                              // share: written and read by this wave alone
   float acc[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll 8
-  for (int s = 0; s < p.nsplit; ++s) {           // share: written and read by this wave alone
+  for (int s = 0; s < p.nsplit; ++s) {
     const float f = share[wave][s];
     const float* q = part + (long)s * step + 2;
 #pragma unroll
