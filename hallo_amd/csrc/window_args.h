@@ -15,7 +15,7 @@ struct WinArgs {
   float scale, c;                                // c = scale * log2(e)
   int nqb;                                       // query blocks of one (batch entry, head)
   // split form (few queries): row blocks of 32 packed rows, key splits, partial results [row block][split][32][hd + 2]
-  int nrb, nsplit; float* part;
+  int nrb, nsplit, Lp; float* part;              // Lp: packed rows of a head
 };
 
 constexpr int WIN_MAX_LEN = 1 << 29;             // sums of two positions / window edges stay inside int

@@ -224,8 +224,10 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-// Few queries.  Row r of a block of 32 is query r % Lq of head hk * group + r / Lq.  Bound by the bytes of K and V: a wave reads 32 keys
-// at a time, whole rows by neighbouring lanes, into LDS tiles of its own (no barrier), the next 32 keys in flight under the products; the four waves take every fourth tile of the split and join through LDS.
+// Few queries.  Packed row r is query r % Lp of head hk * group + r / Lp: Lp = Lq up to 32 queries (a block of 32 rows holds several heads),
+// else the next multiple of 32 (a block over a head's end would walk the keys of all queries).  Bound by the bytes of K and V: a wave reads 32 keys
+// at a time, whole rows by neighbouring lanes, into LDS tiles of its own (no barrier), the next 32 keys in flight under the products; the
+// four waves take every fourth tile of the split and join through LDS.
 // ------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int HK>
 __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
@@ -243,7 +245,7 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   const int rb = bid % p.nrb; bid /= p.nrb;
   const int hk = bid % p.kv_heads, b = bid / p.kv_heads;
   const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk), shift = kn - qn;
-  const int rows = p.group * p.Lq, r = rb * 32 + l31, gh = r / p.Lq, i = r - gh * p.Lq;
+  const int rows = p.group * p.Lp, r = rb * 32 + l31, gh = r / p.Lp, i = r - gh * p.Lp;
   const bool live = r < rows && i < qn;
   const T* K = reinterpret_cast<const T*>(p.k) + (long)b * p.k_bs + (long)hk * p.k_hs;
   const T* V = reinterpret_cast<const T*>(p.v) + (long)b * p.v_bs + (long)hk * p.v_hs;
@@ -255,8 +257,9 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
     qf[ks] = live && d < p.hd ? ld8<T>(Qr + d) : zero8<T>();
   }
   // the queries of this block: all of them once it reaches over a head's end
-  const int last = min(rb * 32 + 31, rows - 1), ilo = rb * 32 / p.Lq == last / p.Lq ? rb * 32 % p.Lq : 0,
-            ihi = min(rb * 32 / p.Lq == last / p.Lq ? last % p.Lq : p.Lq - 1, qn - 1);
+  const int last = min(rb * 32 + 31, rows - 1);
+  const bool one = rb * 32 / p.Lp == last / p.Lp;
+  const int ilo = one ? rb * 32 % p.Lp : 0, ihi = min(one ? last % p.Lp : p.Lp - 1, qn - 1);
   WinRange w = {0, 0, 0};
   if (ihi >= ilo) w = win_range(p, shift + ilo, shift + ihi, kn);
   const int n0 = (w.e0 + 31) / 32, nt = n0 + (w.e1 - w.s1 + 31) / 32;
@@ -378,14 +381,14 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   for (int w4 = 0; w4 < 4; ++w4) Mr = fmaxf(Mr, sm_m[w4][rr]);
 #pragma unroll
   for (int w4 = 0; w4 < 4; ++w4) Lr += sm_l[w4][rr] * (sm_m[w4][rr] == Mr ? 1.0f : __builtin_amdgcn_exp2f((sm_m[w4][rr] - Mr) * c));
-  if (R >= rows) return;
+  const int gr = R / p.Lp, ir = R - gr * p.Lp, h = hk * p.group + gr;
+  if (R >= rows || ir >= p.Lq) return;
   if (p.nsplit > 1) {
     float* part = p.part + (((long)(b * p.kv_heads + hk) * p.nrb + rb) * p.nsplit + split) * 32 * (p.hd + 2) + rr * (p.hd + 2);
     for (int d = cc; d < p.hd; d += 8) part[2 + d] = jt[rr * OP + d];
     if (cc == 0) { part[0] = Mr; part[1] = Lr; }
     return;
   }
-  const int gr = R / p.Lq, ir = R - gr * p.Lq, h = hk * p.group + gr;
   const float inv = Lr > 0.0f ? 1.0f / Lr : (Lr != Lr ? Lr : 0.0f);
   T* O = reinterpret_cast<T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)ir * p.o_rs;
   for (int d = cc * 8; d < p.hd; d += 64) {
@@ -408,7 +411,7 @@ __global__ __launch_bounds__(256) void win_join_kernel(const WinArgs p) {
   const int rows = p.group * p.Lq;
   const long id = (long)blockIdx.x * 4 + wave;
   if (id >= (long)p.batch * p.kv_heads * rows) return;
-  const int R = (int)(id % rows);
+  const int row = (int)(id % rows), gr = row / p.Lq, i = row - gr * p.Lq, R = gr * p.Lp + i;
   const long bh = id / rows;
   const int hk = (int)(bh % p.kv_heads), b = (int)(bh / p.kv_heads);
   const int step = 32 * (p.hd + 2);
@@ -432,7 +435,7 @@ __global__ __launch_bounds__(256) void win_join_kernel(const WinArgs p) {
 #pragma unroll
     for (int k = 0; k < 3; ++k) acc[k] += (lane + 64 * k < p.hd ? q[lane + 64 * k] : 0.0f) * f;
   }
-  const int gr = R / p.Lq, i = R - gr * p.Lq, h = hk * p.group + gr;
+  const int h = hk * p.group + gr;
   const float inv = L > 0.0f ? 1.0f / L : (L != L ? L : 0.0f);
   T* O = reinterpret_cast<T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)i * p.o_rs;
 #pragma unroll
@@ -443,17 +446,25 @@ __global__ __launch_bounds__(256) void win_join_kernel(const WinArgs p) {
 }
 
 // Which form, and how many key splits.
+// The row blocks of the split form have four waves on 32 queries, so a long range takes half as long as in blocks of 128 -- as long as all
+// of them run at once (three per CU up to 64 columns, else two).  Causal, bf16, split form / 128-query blocks: 8192 queries of one head
+// of 64 (256 row blocks) 47 / 151 us, 2 x 1024 of 12 heads of 64 (768) 18 / 24, 1024 of 32 heads (1024) 26 / 25; 1024 of 12 heads of 128
+// (384) 25 / 33, 2 x 1024 of them (768) 41 / 36 us.
 void plan(WinArgs& a) {
   a.nqb = (a.Lq + 127) / 128;
-  a.nrb = (a.group * a.Lq + 31) / 32;
   a.nsplit = 0;                                  // 0: 128-query blocks
-  const long blocks = (long)a.batch * a.heads * a.nqb;
-  if (a.Lq > 32 && blocks >= 128) return;
-  long keys = a.Lk;
-  if (a.left >= 0 && a.right >= 0) keys = (long)a.left + a.right + a.Lq + a.sinks;
+  a.Lp = a.Lq > 32 ? (a.Lq + 31) / 32 * 32 : a.Lq;
+  const long nrb = ((long)a.group * a.Lp + 31) / 32, wgs = (long)a.batch * a.kv_heads * nrb, slots = a.hd <= 64 ? 768 : 512;
+  if (a.Lq > 32 && wgs > slots) return;
+  a.nrb = (int)nrb;
+  long keys = a.Lk;                              // of one row block
+  if (a.left >= 0 && a.right >= 0) keys = (long)a.left + a.right + (a.Lq < 32 ? a.Lq : 32) + a.sinks;
   if (keys > a.Lk) keys = a.Lk;
-  const long wgs = (long)a.batch * a.kv_heads * a.nrb, tiles = (keys + 31) / 32;
-  long ns = (512 + wgs - 1) / wgs;
+  const long tiles = (keys + 31) / 32;
+  // no second round of workgroups for a rest, but where the keys are many: 48 streams of 8 key heads of 128, 16384 keys, one / two
+  // pieces 580 / 535 us; 1024 queries of 12 heads 25 / 37 us; five streams, 12 / 13 pieces of 5000 keys, 29 / 35 us
+  long ns = 512 / wgs;
+  if (ns == 1 && wgs < 512 && tiles >= 128) ns = 2;
   if (ns > tiles / 4) ns = tiles / 4;            // every wave of a split has a tile
   // the second launch and the parts cost what the split saves: one stream of 12 heads of 64 takes 11.4 us against 1024 keys in one piece
   // and in eight, 8.3 and 10.1 us against 512
