@@ -9,6 +9,8 @@
 // (C = 320: 16 lanes x 3 vectors, 4 rows per wave) and a wide one stays in registers (LPR = 256: the whole workgroup on a row).
 // The row sums go through a fixed tree of lane exchanges, the weight gradients through a fixed sequence -- lane, lanes of a wave,
 // waves of a workgroup, workgroups in the second launch -- so a result does not depend on timing (no atomics).
+// 262144 rows of 320, bf16: forward 66 us (5.15 TB/s, as fast as a copy of the same bytes), backward with weight gradients 107 us (4.7 TB/s);
+// 499 rows of 768, fp16: backward 8 + 2 us, two launches.
 #include "common.h"
 #include "../../include/hallo_amd.h"
 

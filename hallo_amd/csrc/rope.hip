@@ -7,7 +7,7 @@
 // Angles: a frequency is a 64-bit fixed-point fraction of a turn, so pos * freq modulo 2^64 IS the angle modulo one turn -- exact for
 // every 32-bit position, where a 32-bit float product is off by whole radians near 10^7.  The top 32 bits go to sincospi.
 //
-// The kernel is bound by HBM (x read once, y written once).  A workgroup takes `tt` tokens: it computes their cos / sin once into LDS,
+// The kernel is bound by HBM (x read once, y written once; 4.5 TB/s on 262144 tokens of 16 heads of 40 in rows of 960, fp16: 149 us).  A workgroup takes `tt` tokens: it computes their cos / sin once into LDS,
 // shared by all heads, then walks (token, head, unit); a unit is V columns and, in the half-split form, their V partners, so every
 // element is read and written by one thread (y may be x).  V = 8 or 4, whichever divides the axes' (half) widths; other widths go
 // through rope_staged_kernel.

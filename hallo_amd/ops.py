@@ -1114,7 +1114,8 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
     j <= p + right, and j >= p - left or j < sinks; a negative left / right means no limit, so the default is causal attention with the
     queries at the end of the keys -- a prompt, a chunk of new tokens, or one new token against a cache of capacity Lk.  q_len / kv_len:
     int32 [B] on the device (default Lq / Lk), clamped to the tensors' lengths.  Queries that see nothing or are padding get zeros.
-    Keys behind kv_len, or outside of every window, may hold anything.  head_dim: a multiple of 8 up to 160.
+    Keys behind kv_len, or outside of every window, may hold anything; a key that some query sees must be finite (others multiply it by 0).
+    head_dim: a multiple of 8 up to 160.  out must not overlap q, k or v.
 
     return_lse: (out, lse), lse fp32 [B, heads, Lq] (-inf where nothing is visible), as window_attention_backward() takes it."""
     _chk_dev(q, k, v, q_len, kv_len, out)
@@ -1138,7 +1139,7 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
 def window_attention_backward(do, q, k, v, o, lse, heads, *, kv_heads=None, left=-1, right=0, sinks=0, q_len=None, kv_len=None, scale=None,
                               dq=None, dk=None, dv=None):
     """(dq, dk, dv) of o, lse = window_attention(q, k, v, ..., return_lse=True) for do, with the same arguments.  dk / dv are summed over
-    the query heads that share a key head; padded rows get zeros.  Results repeat bit for bit."""
+    the query heads that share a key head; padded rows get zeros.  dq / dk / dv must not overlap the inputs.  Results repeat bit for bit."""
     _chk_dev(do, q, k, v, o, lse, q_len, kv_len, dq, dk, dv)
     _like("o", o, q)
     _like("do", do, q)

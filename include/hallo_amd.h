@@ -423,6 +423,7 @@ int hallo_w2v_conv0_gn_gelu(const float* wave, int64_t n_samples, const float* w
 int hallo_lerp_rows(const void* x, void* y, int in_rows, int out_rows, int C, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * (The entry points from here on came without a new version number: nothing before them changed.)
  * LayerNorm for training.  x [rows, C] (row pitch ldx >= C elements, any C in 1 .. 16384, any alignment), stats fp32 [rows][2] =
  * (mean, rstd).  gamma / beta [C] in `dtype`, or fp32 with affine_f32 = 1; null = 1 / 0.
  * hallo_layernorm_train:    y = (x - mean) * rstd * gamma + beta, and stats.  y may be x.
@@ -445,6 +446,7 @@ int hallo_layernorm_backward(const void* dy, int64_t lddy, const void* x, int64_
  * (i, i + dims[a] / 2).  Columns behind the last axis are copied.  head_dim even, at most 256.
  * Positions: pos int32 [batch or 1, L, n_axes] (pos_bs = 0: one row for all entries), or pos = null and a grid whose cells are the L
  * tokens, the last axis fastest, counted from origin.  inverse = 1: negative angles, which is the gradient.  y may be x (same strides).
+ * At most 2^16 heads; L below 2^31 - 64.
  */
 typedef struct hallo_rope_desc {
   const void* x; void* y;
@@ -464,7 +466,8 @@ int hallo_rope(const hallo_rope_desc* d, void* stream);
  * p = kv_len[b] - q_len[b] + i and sees key j iff j < kv_len[b], j <= p + right (right < 0: no limit), and j >= p - left (left < 0: no
  * limit) or j < sinks.  q [batch, Lq, heads, head_dim], k / v [batch, Lk, kv_heads, head_dim] with heads % kv_heads == 0 (query head h
  * reads key head h / (heads / kv_heads)), o like q; strides in elements, multiples of 8, row strides at most 2^24, 16-byte aligned bases;
- * head_dim % 8 == 0, at most 160; lengths at most 2^29.
+ * head_dim % 8 == 0, at most 160; lengths at most 2^29; scale 1e-30 .. 1e30.  o must not overlap the inputs, nor its rows one another.
+ * V rows that some queries of a tile see and others do not are multiplied by 0 for the latter: they must be finite.
  * q_len / kv_len: int32 [batch] on the device, clamped to 0 .. Lq / Lk; null = Lq / Lk.  A query that sees nothing, and one at or behind
  * q_len, gets zeros and lse = -inf.  lse (may be null): fp32 [batch, heads, Lq], natural logarithm of the row's sum.
  * What lies at or behind kv_len, or outside of every query's window, is not used and may hold anything.
@@ -472,7 +475,7 @@ int hallo_rope(const hallo_rope_desc* d, void* stream);
  *
  * hallo_window_attention_backward: dq, dk, dv for dout, with q, k, v, o, lse and the mask as in `fwd` (fwd.o and fwd.lse are read; lse
  * must be there).  dk / dv are summed over the query heads of a key head; rows at or behind q_len / kv_len are written as zeros.
- * Deterministic.  fwd.workspace: hallo_window_attention_backward_workspace(d) bytes.
+ * dq, dk, dv must overlap neither the inputs nor one another.  Deterministic.  fwd.workspace: hallo_window_attention_backward_workspace(d) bytes.
  */
 typedef struct hallo_window_attn_desc {
   const void* q; const void* k; const void* v; void* o;
