@@ -13,7 +13,7 @@
 //
 // What bounds them: win_fwd_kernel the SIMDs' issue -- MFMA and vector time (exponentials, maxima, sums, conversions) add up rather than
 // overlap, 39 + 39 % of all cycles at 128 columns, 41 + 50 % at 80, the LDS port 30 - 35 % busy.  2 x 8192 tokens, 32 / 8 heads of 128,
-// window 4096, bf16: 0.97 ms, 855 TFLOP/s; 2 x 16384 tokens, 8 heads of 80, 4097 + 1024 keys a token, fp16: 0.56 ms, 700 TFLOP/s.
+// window 4096, bf16: 0.95 ms, 868 TFLOP/s; 2 x 16384 tokens, 8 heads of 80, 4097 + 1024 keys a token, fp16: 0.55 ms, 723 TFLOP/s.
 // win_split_kernel the bytes of K and V: 32 streams, 16 k window, 8 key heads of 128: 0.36 ms, 5.75 TB/s.
 #include <type_traits>
 #include "window_args.h"

@@ -11,7 +11,7 @@
 //          (also used for all keys when there are too few key tiles to fill the chip, and for dq's keys when there are few queries)
 // S and dO V^T are computed in both dkv and dq (7 products where 5 would do with atomics on dQ): results do not depend on timing.
 // Bound by the SIMDs' issue as the forward pass (MFMA 40 %, vector 30 - 33 % of all cycles, LDS port 27 - 37 % busy).  2 x 8192 tokens, 32 / 8
-// heads of 128, window 4096, bf16: 3.25 ms (dkv 1.84, dq 1.41, prep 0.06), 635 TFLOP/s of the five products that count, 890 of the seven done.
+// heads of 128, window 4096, bf16: 3.2 ms (dkv 1.79, dq 1.38, prep 0.06), 640 TFLOP/s of the five products that count, 900 of the seven done.
 //
 // fp16: P is 1/N over long rows and dS smaller still, below fp16's normal numbers.  Both are carried scaled by powers of two that cannot
 // overflow and are taken out of the fp32 accumulators at the end: P by 2^14 (P <= 1), dS by 2^e with |dS| = P |do_i . (v_j - o_i)| <=
@@ -148,13 +148,15 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
   const int hi = lane >> 5, l31 = lane & 31, kg = wave & 3;
   const bool role = wave >> 2;
 
-  // block -> (key head, batch entry, key tile, query split); the longest tiles (sinks, then the first keys) come first
+  // block -> (key head, batch entry, key tile, query split); the longest tiles come first: the sinks, then the first keys, or the last
+  // ones where the queries see everything ahead of them but not everything behind
   int bid = blockIdx.x;
   const int hk = bid % p.kv_heads; bid /= p.kv_heads;
   const int b = bid % p.batch; bid /= p.batch;
   const bool sink = bid < a.nst * a.sps;
   const int loc = sink ? bid : bid - a.nst * a.sps, sp = sink ? a.sps : a.spr;
-  const int tile = loc / sp, split = loc - tile * sp;
+  const int order = loc / sp, split = loc - order * sp;
+  const int tile = !sink && p.right < 0 && p.left >= 0 ? a.nrt - 1 - order : order;
   const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk), shift = kn - qn;
   const int s_end = min(p.sinks, p.Lk);
   const int ka = (sink ? 0 : s_end) + tile * BW_KEYS, kz = min(ka + BW_KEYS, sink ? s_end : p.Lk), kb = min(kz, kn);
@@ -341,7 +343,7 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
   }
   float* part = nullptr;
   if (sp > 1) {
-    const int tp = sink ? loc : (a.sps > 1 ? a.nst * a.sps : 0) + loc;
+    const int tp = (sink || a.sps == 1 ? 0 : a.nst * a.sps) + tile * sp + split;
     part = a.part + (((long)b * p.kv_heads + hk) * a.nparts + tp) * BW_KEYS * 2 * p.hd + (role ? 0 : p.hd);
   }
   T* D = role ? reinterpret_cast<T*>(a.dk) + (long)b * a.dk_bs + (long)hk * a.dk_hs
@@ -379,15 +381,19 @@ __global__ __launch_bounds__(256) void win_bwd_join_kernel(const WinBwdArgs a) {
   const float* part = a.part + (((long)b * p.kv_heads + hk) * a.nparts + tp) * BW_KEYS * 2 * p.hd;
   T* dK = reinterpret_cast<T*>(a.dk) + (long)b * a.dk_bs + (long)hk * a.dk_hs;
   T* dV = reinterpret_cast<T*>(a.dv) + (long)b * a.dv_bs + (long)hk * a.dv_hs;
-  const int w = 2 * p.hd;
-  for (int k = threadIdx.x; k < 8 * w; k += 256) {
-    const int kl = rows8 * 8 + k / w, d = k % w, j = ka + kl;
+  using V4 = typename Vec<T>::v4;
+  const int w = 2 * p.hd, w4 = w / 4;            // four columns per thread
+  for (int k = threadIdx.x; k < 8 * w4; k += 256) {
+    const int r = k / w4, d = (k - r * w4) * 4, kl = rows8 * 8 + r, j = ka + kl;
     if (j >= kz) continue;
-    float s = 0.0f;
+    const float* q = part + (long)kl * w + d;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
-    for (int i = 0; i < sp; ++i) s += part[(long)i * BW_KEYS * w + (long)kl * w + d];
-    if (d < p.hd) dK[(long)j * a.dk_rs + d] = from_f32<T>(s);
-    else dV[(long)j * a.dv_rs + d - p.hd] = from_f32<T>(s);
+    for (int i = 0; i < sp; ++i) s += *reinterpret_cast<const f32x4*>(q + (long)i * BW_KEYS * w);
+    V4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = from_f32<T>(s[e]);
+    *reinterpret_cast<V4*>(d < p.hd ? dK + (long)j * a.dk_rs + d : dV + (long)j * a.dv_rs + d - p.hd) = x;
   }
 }
 
@@ -592,10 +598,14 @@ __global__ __launch_bounds__(256) void win_bwd_join_q_kernel(const WinBwdArgs a)
   *reinterpret_cast<V4*>(reinterpret_cast<T*>(a.dq) + (long)b * a.dq_bs + (long)h * a.dq_hs + (long)i * a.dq_rs + d) = w;
 }
 
-// Key tiles and query splits.  A sink tile meets every query, a tile of the rest at most left + right + 128 of them, and there may be fewer
-// tiles than the chip takes at once: queries are split so that a workgroup has at most `target` steps of 32 query rows, the least
-// number of steps with which all workgroups run at once (two per CU up to 64 columns, else one).  Below 8 steps the parts cost more than
-// they save.
+// Key tiles and query splits.  A sink tile meets every query, a tile of the rest at most left + right + 128 of them, one of a triangle half
+// as many on average, and there may be fewer tiles than the chip takes at once (two workgroups per CU up to 64 columns, else one): queries
+// are split so that a workgroup has at most `target` steps of 32 query rows (about 1 us each), with the least of
+//   one round: the longest workgroup;   more: all steps / slots + a quarter of the longest (the longest go first),
+// a workgroup counting 8 steps more than it has and, with parts to write and to join, 20 (13 where all write at once).  Measured, dkv and
+// join: 2 x 2048 causal, 32 / 8 heads of 128, whole / two parts 262 / 177 us; 5 x 7047 without a left edge, 8 heads on one of 128, whole /
+// five parts 1765 / 740 us; 5 x 972, 8 / 4 heads of 80, whole / two / three parts 65 / 47 / 53 us; 4 x 1024, 12 heads of
+// 64, whole / two parts 44 / 48 us.
 int64_t plan_bwd(WinBwdArgs& a) {
   WinArgs& p = a.w;
   p.nqb = (p.Lq + 127) / 128;
@@ -610,17 +620,35 @@ int64_t plan_bwd(WinBwdArgs& a) {
   if (p.left >= 0 && p.right >= 0 && (long)p.left + p.right + BW_KEYS < span) span = (long)p.left + p.right + BW_KEYS;
   const long it_s = (long)p.group * ((p.Lq + 31) / 32), it_r = (long)p.group * ((span + 31) / 32);
   const auto parts = [](long its, long target) { const long n = (its + target - 1) / target; return n < 1 ? 1L : n; };
-  long target = 8;
-  while (target < it_r && bh * (a.nst * parts(it_s, target) + a.nrt * parts(it_r, target)) > slots) target += (target + 7) / 8;
-  if (target > it_r) target = it_r;              // more tiles than slots: only the sinks are split, into pieces as long as the others
-  if (target < 8) target = 8;
+  long sum = 0, seen = 0;                        // mean span over up to 64 tiles
+  const long shift = (long)p.Lk - p.Lq;
+  for (long t = 0, dt = a.nrt / 64 + 1; t < a.nrt; t += dt, ++seen) {
+    const long ka = s_end + t * BW_KEYS, kb = ka + BW_KEYS < p.Lk ? ka + BW_KEYS : p.Lk;
+    const long ia = p.right < 0 ? 0 : ka - p.right - shift, ib = p.left < 0 ? p.Lq : kb + p.left - shift;
+    const long n = (ib < p.Lq ? ib : p.Lq) - (ia > 0 ? ia : 0);
+    sum += n > 0 ? n : 0;
+  }
+  const double all = bh * ((double)a.nst * it_s + (seen ? (double)a.nrt * p.group * sum / (32.0 * seen) : 0.0));
+  const long most = a.nst && it_s > it_r ? it_s : it_r;
+  long target = most;
+  double best = 1e300;
+  for (long t = 8;; t += (t + 7) / 8) {
+    const long ns = parts(it_s, t), nr = parts(it_r, t), wgs = bh * (a.nst * ns + a.nrt * nr), longest = t < most ? t : most;
+    const bool joined = (a.nst && ns > 1) || nr > 1;
+    const double extra = joined ? 20.0 : 8.0;
+    const double cost = wgs <= slots ? longest + (joined ? 13.0 : 8.0) : (all + wgs * extra) / slots + (longest + extra) / 4;
+    if (cost < best) { best = cost; target = t; }
+    if (t >= most) break;
+  }
   a.sps = a.nst ? (int)parts(it_s, target) : 1;
   a.spr = a.nrt ? (int)parts(it_r, target) : 1;
-  // dq: few queries leave CUs idle, then the keys are split (two workgroups per CU, at least 8 tiles of 32 keys each)
+  // dq: few queries leave CUs idle, then the keys are split (up to 64 columns four workgroups per CU, else two, at least 8 tiles of 32 keys
+  // each; 6 x 190 x 3062, 28 heads of 40: 112 -> 61 us and 5 for the join)
   long keys = p.Lk;
   if (p.left >= 0 && p.right >= 0 && (long)p.left + p.right + p.Lq + p.sinks < keys) keys = (long)p.left + p.right + p.Lq + p.sinks;
   const long blocks = (long)p.batch * p.heads * p.nqb, tiles = (keys + 31) / 32;
-  long sq = blocks > 0 && blocks < 256 ? 512 / blocks : 1;
+  const long want = p.hd <= 64 ? 1024 : 512;
+  long sq = blocks > 0 && blocks < want / 2 ? want / blocks : 1;
   if (sq > tiles / 8) sq = tiles / 8;
   a.spq = sq < 1 ? 1 : (int)sq;
   a.nparts = (a.sps > 1 ? a.nst * a.sps : 0) + (a.spr > 1 ? a.nrt * a.spr : 0);
