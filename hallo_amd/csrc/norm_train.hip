@@ -266,11 +266,13 @@ __global__ __launch_bounds__(1024) void ln_bwd_join_kernel(const float* __restri
 // Lanes per row and vectors per lane for a row of nvec vectors: the fewest lanes that hold it with at most 3 vectors each, past 192
 // vectors the whole workgroup.  3 is for the backward pass -- x and dy twice (now and next), gamma and both gradients in registers --
 // on 262144 rows of 320 (bf16): 16 lanes x 3 (a sixth of them idle) 107 us, 8 lanes x 5 (none idle, one wave per SIMD) 147 us.
-void pick(int nvec, bool al, int& lpr, int& vpl) {
+// Rows that 16 lanes or more hold with 2 take 3 all the same: 262144 rows of 256, fp16, backward 89 us against 93 (forward 42.5 both).  Past 8
+// lanes only: 197031 rows of 50, 8 lanes x 1 / x 3, 25 / 50 us.
+void pick(int nvec, int& lpr, int& vpl) {
   if (nvec > 192) { lpr = 256; vpl = nvec <= 512 ? 2 : (nvec <= 1024 ? 4 : 8); return; }
   lpr = 8;
   while (lpr * 3 < nvec) lpr *= 2;
-  vpl = lpr > 8 || !al ? 3 : (nvec + lpr - 1) / lpr;       // rows that are not 16-byte aligned: one form per lane count
+  vpl = lpr > 8 ? 3 : (nvec + lpr - 1) / lpr;
 }
 
 constexpr int LN_MAX_C = 16384;
@@ -290,7 +292,7 @@ int launch_fwd(const void* x, int64_t ldx, void* y, int64_t ldy, const void* g, 
                float eps, hipStream_t st) {
   const bool al = C % 8 == 0 && aligned16(x, ldx) && aligned16(y, ldy);
   int lpr, vpl;
-  pick((C + 7) / 8, al, lpr, vpl);
+  pick((C + 7) / 8, lpr, vpl);
   const int64_t grid = (rows * lpr + 255) / 256;
   if (grid > 0x7fffffff) return -22;
   auto go = [&](auto L, auto V, auto A) {
@@ -313,7 +315,7 @@ int launch_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const fl
                float* dgamma, float* dbeta, float* parts, int64_t rows, int C, hipStream_t st) {
   const bool al = C % 8 == 0 && aligned16(x, ldx) && aligned16(dy, ldd) && aligned16(dx, lddx);
   int lpr, vpl;
-  pick((C + 7) / 8, al, lpr, vpl);
+  pick((C + 7) / 8, lpr, vpl);
   const int wgs = bwd_wgs(rows, lpr);
   const bool direct = wgs == 1 && dgamma && dbeta == dgamma + C;     // one workgroup: its sums are the result
   float* to = direct ? dgamma : parts;
@@ -359,7 +361,7 @@ extern "C" int64_t hallo_layernorm_backward_workspace(int64_t rows, int C) {
   using namespace hallo;
   if (rows < 0 || C < 1 || C > LN_MAX_C) return -22;
   int lpr, vpl;
-  pick((C + 7) / 8, true, lpr, vpl);
+  pick((C + 7) / 8, lpr, vpl);
   return (int64_t)bwd_wgs(rows, lpr) * 2 * C * 4;
 }
 
