@@ -247,8 +247,8 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   const int hi = lane >> 5, l31 = lane & 31;
   int bid = blockIdx.x;
   const int split = bid % p.nsplit; bid /= p.nsplit;
-  const int rb = bid % p.nrb; bid /= p.nrb;
-  const int hk = bid % p.kv_heads, b = bid / p.kv_heads;
+  const int hk = bid % p.kv_heads; bid /= p.kv_heads;
+  const int b = bid % p.batch, rb = p.nrb - 1 - bid / p.batch;         // causal masks: the row blocks with the most keys first
   const int qn = win_len(p.q_len, b, p.Lq), kn = win_len(p.kv_len, b, p.Lk), shift = kn - qn;
   const int rows = p.group * p.Lp, r = rb * 32 + l31, gh = r / p.Lp, i = r - gh * p.Lp;
   const bool live = r < rows && i < qn;
@@ -452,14 +452,18 @@ __global__ __launch_bounds__(256) void win_join_kernel(const WinArgs p) {
 
 // Which form, and how many key splits.
 // The row blocks of the split form have four waves on 32 queries, so a long range takes half as long as in blocks of 128 -- as long as all
-// of them run at once (three per CU up to 64 columns, else two).  Causal, bf16, split form / 128-query blocks: 8192 queries of one head
-// of 64 (256 row blocks) 47 / 151 us, 2 x 1024 of 12 heads of 64 (768) 18 / 24, 1024 of 32 heads (1024) 26 / 25; 1024 of 12 heads of 128
-// (384) 25 / 33, 2 x 1024 of them (768) 41 / 36 us.
+// of them run at once (three per CU up to 64 columns, else two; under a causal mask half of the keys on average and the longest first, so
+// half as many again, twice as many where a workgroup is long).  Causal, bf16, split form / 128-query blocks: 8192 queries of one head of 64
+// (256 row blocks) 40 / 151 us, 2 x 2048 of 8 heads of 64 (1024) 30 / 43 us; of 128 columns: 1024 of 12 heads (384) 21 / 33, 2 x 1024 of
+// them (768) 31 / 36, 8192 of four heads (1024) 154 / 247, 1024 of 32 heads (1024) 38 / 34 us.  +- 100 keys, 4 x 500 of 12 heads (768):
+// 64 columns 11 / 13, 128 columns 21 / 18 us.
 void plan(WinArgs& a) {
   a.nqb = (a.Lq + 127) / 128;
   a.nsplit = 0;                                  // 0: 128-query blocks
   a.Lp = a.Lq > 32 ? (a.Lq + 31) / 32 * 32 : a.Lq;
-  const long nrb = ((long)a.group * a.Lp + 31) / 32, wgs = (long)a.batch * a.kv_heads * nrb, slots = a.hd <= 64 ? 768 : 512;
+  const bool causal = a.left < 0 && a.right >= 0 && a.right < a.Lk / 2 && a.Lk < 2L * a.Lq;
+  const long nrb = ((long)a.group * a.Lp + 31) / 32, wgs = (long)a.batch * a.kv_heads * nrb;
+  const long slots = causal && a.Lk >= 2048 ? 1024 : a.hd <= 64 || causal ? 768 : 512;
   if (a.Lq > 32 && wgs > slots) return;
   a.nrb = (int)nrb;
   long keys = a.Lk;                              // of one row block
