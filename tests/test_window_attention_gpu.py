@@ -412,3 +412,16 @@ def test_other_stream():
         g = ops.window_attention_backward(do, q, k, v, o, l2, 4, **kw)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(o, want) and torch.equal(l2, lse) and all(torch.equal(a, b) for a, b in zip(g, grads))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,hd,left,right,sinks", [
+    (6, 2100, 2100, 2, 2, 64, -1, 0, 0),         # row blocks of 32 queries under a long causal mask, more of them than run at once
+    (1, 1100, 1100, 8, 2, 128, -1, 0, 0),        # dK / dV in parts, keys of a triangle
+    (2, 1100, 1100, 4, 2, 80, 40, -1, 200),      # no right edge: the last keys have the most queries; sinks and the rest in parts
+    (1, 90, 2500, 14, 2, 40, -1, 3, 0),          # heads of 90 queries packed to 96 rows, keys of dq split
+    (3, 70, 1300, 4, 1, 160, 1000, 0, 5),
+])
+def test_plans(dtype, B, Lq, Lk, H, Hkv, hd, left, right, sinks):
+    """Sizes that take each way of dividing the work."""
+    _both(B, Lq, Lk, H, Hkv, hd, dtype, left, right, sinks, _lens(*[Lq - 5 * b for b in range(B)]), _lens(*[Lk - 7 * b for b in range(B)]))
