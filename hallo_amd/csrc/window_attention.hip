@@ -2,8 +2,8 @@
 //
 // Two forms.  `win_fwd_kernel` takes 128 queries of one head per workgroup (a wave owns 32) and walks the keys those queries see; K and
 // V tiles go global -> registers -> LDS one tile ahead of the MFMAs.  `win_split_kernel` is for few queries (single tokens against a
-// cache): the query rows of the heads that share a key head are packed into one 32-row block, the keys are split over workgroups and
-// over the waves of each, and `win_join_kernel` joins the parts.
+// cache, prompts of few heads): the query rows of the heads that share a key head are packed into 32-row blocks, the keys are split over
+// workgroups and over the waves of each, and `win_join_kernel` joins the parts.
 //
 // Both contractions run in swapped form, so a lane owns a query and the softmax statistics are lane-local:
 //   S^T[key, q] = K[key, :] . Q[q, :]      A = K rows from LDS, B = Q fragments in registers
