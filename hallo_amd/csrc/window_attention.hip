@@ -9,7 +9,11 @@
 //   S^T[key, q] = K[key, :] . Q[q, :]      A = K rows from LDS, B = Q fragments in registers
 //   O^T[d, q]   = V^T[d, :] . P^T[:, q]    A = V read transposed from LDS, B = P as the first product left it
 // The running maximum moves only when a score exceeds it by more than 6 (log2 units, so P <= 64 and the row sum stays far inside
-// fp32); P is rounded to the storage type for the second product only -- the row sum adds the unrounded values.
+// fp32).  P is rounded to the storage type for the second product only, because the matrix cores take 16-bit operands at the rate that
+// this kernel lives on; the row sum adds the unrounded values, so a rounding is a relative error of half a step in one weight.  fp16's
+// smallest number would make it more than that: thousands of weights below 2^-25 of the largest one would be in the sum and not in the
+// product.  P therefore carries a power of two that rides in the exponent and leaves with the division by the sum (fp16, win_fwd_kernel:
+// 2^9, 64 * 2^9 is half of fp16's range; win_split_kernel, whose P is at most 1: 2^14; bf16 has fp32's range: none).
 //
 // What bounds them: win_fwd_kernel the SIMDs' issue -- MFMA and vector time (exponentials, maxima, sums, conversions) add up rather than
 // overlap, 39 + 39 % of all cycles at 128 columns, 41 + 50 % at 80, the LDS port 30 - 35 % busy.  2 x 8192 tokens, 32 / 8 heads of 128,
@@ -23,6 +27,8 @@ namespace hallo {
 
 namespace {
 
+constexpr float FWD_P_EXP = 9.0f, SPLIT_P_EXP = 14.0f;       // fp16: exponent of the power of two that P carries
+
 template <typename T, int HK>
 __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
   using V8 = typename Vec<T>::v8;
@@ -32,7 +38,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
   using Tile = WinTile<HK>;
   constexpr int TB = KB * Tile::PITCH, STAGE = 2 * TB;   // K | V
   constexpr int U = (KB * CH + 255) / 256;       // 16-byte pieces per thread and tensor
-  constexpr float NEG_INF = -__builtin_inff();
+  constexpr float NEG_INF = -__builtin_inff(), X = std::is_same<T, _Float16>::value ? FWD_P_EXP : 0.0f;
   __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
   win_lds* const lds = (win_lds*)smem;
 
@@ -172,7 +178,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[db][e] *= a;
       }
-      const float mc = m == NEG_INF ? 0.0f : m * c;
+      const float mc = (m == NEG_INF ? 0.0f : m * c) - X;
       V8 pf[NT][2];
       float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -212,7 +218,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
   // a NaN sum stays NaN
   const float inv = some ? 1.0f / l : (l != l && row < qn ? l : 0.0f);
   if (p.lse && hi == 0)
-    p.lse[((long)b * p.heads + h) * p.Lq + row] = some ? (m * c + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f : (inv != 0.0f ? inv : NEG_INF);
+    p.lse[((long)b * p.heads + h) * p.Lq + row] = some ? (m * c + (__builtin_amdgcn_logf(l) - X)) * 0.69314718055994530942f : (inv != 0.0f ? inv : NEG_INF);
   T* O = reinterpret_cast<T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)row * p.o_rs;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
@@ -238,7 +244,9 @@ template <typename T, int HK>
 __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   using V8 = typename Vec<T>::v8;
   constexpr int NKS = HK / 16, NDB = (HK + 31) / 32, OP = HK + 4;      // OP: pitch of the joined rows, floats
-  constexpr float NEG_INF = -__builtin_inff();
+  constexpr bool F16 = std::is_same<T, _Float16>::value;
+  constexpr float NEG_INF = -__builtin_inff(), X = F16 ? SPLIT_P_EXP : 0.0f, UNDO = F16 ? 0x1p-14f : 1.0f;
+  static_assert(SPLIT_P_EXP == 14.0f, "UNDO");
   using Tile = WinTile<HK, HK == 112 || HK == 128 ? 16 : win_chunks(HK)>;      // eight tiles of a workgroup: two workgroups per CU at 128 columns
   constexpr int TB = 32 * Tile::PITCH, WT = 4 * 2 * TB, JT = 32 * OP * 4;      // LDS: K | V of every wave, then the joined rows
   __shared__ __attribute__((aligned(16))) unsigned char smem[WT > JT ? WT : JT];
@@ -339,7 +347,7 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[db][e] *= a;
     }
-    const float mc = m == NEG_INF ? 0.0f : m * c;
+    const float mc = (m == NEG_INF ? 0.0f : m * c) - X;
     V8 pf[2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -353,12 +361,12 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
       for (int h2 = 0; h2 < 2; ++h2) o[db] = Vec<T>::mfma32(tl.template col<V8>(vt, h2 * 16, db), pf[h2], o[db]);
     wave_lds_order();
   }
-  l = win_half_sum(l);
+  l = win_half_sum(l) * UNDO;
   if (!live) { m = NEG_INF; l = 0.0f; }          // rows without a query went along in the tiles that need no mask
   if (hi == 0) { sm_m[wave][l31] = m; sm_l[wave][l31] = l; }
   __syncthreads();                               // also: every wave is done with its V tile, the joined rows take its place
   const float M = fmaxf(fmaxf(sm_m[0][l31], sm_m[1][l31]), fmaxf(sm_m[2][l31], sm_m[3][l31]));
-  const float f = m == M ? 1.0f : __builtin_amdgcn_exp2f((m - M) * c);        // this wave's share (a wave without a visible key: o = 0)
+  const float f = UNDO * (m == M ? 1.0f : __builtin_amdgcn_exp2f((m - M) * c));       // this wave's share (a wave without a visible key: o = 0)
   float* const jt = reinterpret_cast<float*>(smem);
   for (int w4 = 0; w4 < 4; ++w4) {
     if (wave == w4) {
