@@ -38,6 +38,12 @@ __device__ __forceinline__ WinRange win_range(const WinArgs& p, int plo, int phi
   return lo <= se ? WinRange{hi, hi, hi} : WinRange{se, lo, hi};
 }
 
+// largest of the row norms n[i], one for every 64 rows, over the rows lo .. hi - 1 and those beside them in their blocks
+__device__ __forceinline__ float win_norm(const float* n, int lo, int hi, int lane, float big) {
+  for (int i = lo / 64 + lane; i * 64 < hi; i += 64) big = fmaxf(big, n[i]);
+  return big;
+}
+
 // LDS tiles of rows of HK elements (a multiple of 16): rows of C 16-byte chunks, chunk c of row r stored at c ^ swz(r).  A tile is read
 // along its rows (MFMA operand, 16 bytes per lane, lane = row: 16 consecutive rows at one chunk) and transposed (32 lanes: 4 consecutive
 // rows x 64 aligned bytes); the swizzle puts both kinds of 256 bytes on all 64 banks once.  It repeats every 16 rows, so a fragment

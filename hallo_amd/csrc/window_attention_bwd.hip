@@ -15,8 +15,10 @@
 //
 // fp16: P is 1/N over long rows and dS smaller still, below fp16's normal numbers.  Both are carried scaled by powers of two that cannot
 // overflow and are taken out of the fp32 accumulators at the end: P by 2^14 (P <= 1), dS by 2^e with |dS| = P |do_i . (v_j - o_i)| <=
-// 2 |do_i|_2 max_j |v_j|_2 < 2^(15 - e) -- in dkv with the largest |do_i| of the group, in dq with the lane's own do row.  (A key's own
-// |v_j| bounds nothing: o_i is as long as the longest v.)  bf16 has fp32's range and needs neither.
+// 2 |do_i|_2 max_j |v_j|_2 < 2^(15 - e) -- in dkv with the largest |do_i| of the group's queries that see the tile, in dq with the lane's
+// own do row, and j over the keys that these queries see.  (A key's own |v_j| bounds nothing: o_i is as long as the longest v that i sees.
+// The largest over the whole sequence would do, and lose what is small behind a window in fp16's subnormal numbers.)  bf16 has fp32's range
+// and needs neither.
 #include <type_traits>
 #include "window_args.h"
 #include "../../include/hallo_amd.h"
@@ -184,10 +186,12 @@ __global__ __launch_bounds__(512, HK <= 64 ? 4 : 2) void win_bwd_dkv_kernel(cons
   float g = 1.0f;                                // fp16: scale of dS
   if (F16 && role) {
     float dm = 0.0f, vm = 0.0f;
-    const float* m = a.domax + ((long)b * p.heads + hk * p.group) * a.nq64;
-    const float* n = a.vmax + ((long)b * p.kv_heads + hk) * a.nk64;
-    for (int i = lane; i < p.group * a.nq64; i += 64) dm = fmaxf(dm, m[i]);
-    for (int i = lane; i < a.nk64; i += 64) vm = fmaxf(vm, n[i]);
+    if (ib > ia) {
+      const WinRange r = win_range(p, shift + ia, shift + ib - 1, kn);
+      const float* n = a.vmax + ((long)b * p.kv_heads + hk) * a.nk64;
+      vm = win_norm(n, r.s1, r.e1, lane, win_norm(n, 0, r.e0, lane, 0.0f));
+      for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) dm = win_norm(a.domax + ((long)b * p.heads + h) * a.nq64, ia, ib, lane, dm);
+    }
     g = ds_scale(wave_max(dm), wave_max(vm));
   }
   const float gs = g * 0x1p-14f;                 // relative to P's
@@ -440,19 +444,16 @@ __global__ __launch_bounds__(256, 2) void win_bwd_dq_kernel(const WinBwdArgs a) 
   const long at = ((long)b * p.heads + h) * p.Lq + row;
   float lse = row < qn ? a.lse2[at] : __builtin_inff();
   const float delta = row < qn ? a.delta[at] : 0.0f;
+  WinRange r = {0, 0, 0};
+  if (i0 < qn) r = win_range(p, shift + i0, shift + min(i0 + 127, qn - 1), kn);
   float undo = p.scale;
   if (F16) {                                     // the scale of dS rides in the exponent of P
-    float vm = 0.0f;
-    const float* m = a.vmax + ((long)b * p.kv_heads + hk) * a.nk64;
-    for (int i = lane; i < a.nk64; i += 64) vm = fmaxf(vm, m[i]);
-    vm = wave_max(vm);
+    const float* n = a.vmax + ((long)b * p.kv_heads + hk) * a.nk64;
+    const float vm = wave_max(win_norm(n, r.s1, r.e1, lane, win_norm(n, 0, r.e0, lane, 0.0f)));
     const float g = ds_scale(sqrtf(win_half_sum(gsq)), vm);
     lse -= __builtin_amdgcn_logf(g);
     undo = p.scale / g;
   }
-
-  WinRange r = {0, 0, 0};
-  if (i0 < qn) r = win_range(p, shift + i0, shift + min(i0 + 127, qn - 1), kn);
   const int n0 = (r.e0 + KB - 1) / KB, all_t = n0 + (r.e1 - r.s1 + KB - 1) / KB;
   const int tb = (int)((long)all_t * split / a.spq), nt = (int)((long)all_t * (split + 1) / a.spq);      // tiles tb .. nt - 1
   const int pw0 = shift + iw, pw1 = shift + min(iw + 31, qn - 1), pos = shift + row;
