@@ -342,6 +342,16 @@ extern "C" int hallo_rope(const hallo_rope_desc* d, void* stream) {
   const long width = (long)d->heads * d->head_dim;
   if (d->x_rs < 0 || d->y_rs < width || d->L > 0x7fffffff - ROPE_TT || (d->batch > 0 && d->L > (1L << 46) / d->batch)) return -22;
   if (none) return 0;
+  if (d->batch > 1) {                            // rows of different entries must not share elements: two workgroups would write them
+    const int64_t ext = d->L > 1 ? (d->L - 1) * d->y_rs + width : width;
+    if (d->y_bs < ext) {
+      if (d->L == 1 || d->y_bs < width) return -22;
+      for (int64_t b = 1; b < d->batch && b * d->y_bs / d->y_rs < d->L; ++b) {
+        const int64_t l = b * d->y_bs / d->y_rs, rest = b * d->y_bs % d->y_rs;
+        if (rest < width || (l + 1 < d->L && d->y_rs - rest < width)) return -22;
+      }
+    }
+  }
   if (!d->x || !d->y || !d->freq) return -22;
   if (d->x == d->y && (d->x_bs != d->y_bs || d->x_rs != d->y_rs)) return -22;
   a.x = d->x; a.y = d->y;

@@ -981,6 +981,21 @@ class RopeAxes:
         self.freq = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64).to(device)
 
 
+def _entries_meet(B, L, bs, rs, W):
+    """Whether rows of different batch entries share elements: rows of W at b * bs + l * rs, rs >= W."""
+    if bs >= (L - 1) * rs + W if L > 1 else bs >= W:
+        return False
+    if L == 1 or bs < W:
+        return True
+    for b in range(1, B):                        # entry b against entry 0, row 0 of either
+        l, rest = divmod(b * bs, rs)
+        if l >= L:
+            break
+        if rest < W or (l + 1 < L and rs - rest < W):
+            return True
+    return False
+
+
 def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
     """Rotary positions on x [B, L, heads * head_dim] (any batch / row stride: column slices of a fused q|k|v buffer, q|k together).
 
@@ -1001,7 +1016,7 @@ def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
     if L >= 2 ** 31 - 64 or W // hd > 1 << 16:
         _bad(f"x: at most 2^31 - 65 tokens of 2^16 heads, got {tuple(sh)}")
     so = out.stride()
-    if so[2] != 1 or (L > 1 and so[1] < W) or (B > 1 and L and not so[0]):
+    if so[2] != 1 or (L > 1 and so[1] < W) or (B > 1 and L and _entries_meet(B, L, so[0], so[1], W)):
         _bad(f"out: expected {tuple(sh)} with rows that do not overlap, got {tuple(out.shape)} strides {so}")
     if (pos is None) == (grid is None):
         _bad("give either pos or grid")
