@@ -332,7 +332,7 @@ extern "C" int hallo_rope(const hallo_rope_desc* d, void* stream) {
     g = gcd(g, il ? d->dims[i] : d->dims[i] / 2);
     a.dims[i] = d->dims[i];
     if (!d->pos && !none) {
-      if (d->grid[i] < 1 || cells > d->L / d->grid[i] + 1) return -22;
+      if (d->grid[i] < 1 || cells > d->L / d->grid[i] + 1 || (int64_t)d->origin[i] + d->grid[i] > 1LL << 31) return -22;
       cells *= d->grid[i];
       a.grid[i] = d->grid[i];
       a.origin[i] = d->origin[i];

@@ -42,3 +42,11 @@ def test_rope_abi_entries_on_one_another(lib):  # noqa: F811
     for kw in (dict(y_bs=0), dict(y_bs=40), dict(y_bs=200), dict(y_bs=-240), dict(y_bs=100, y_rs=80), dict(y_bs=39, y_rs=80)):
         assert call(**kw) == -22, kw
     del keep
+
+
+def test_rope_abi_positions_past_32_bits(lib):  # noqa: F811
+    keep, p = _mem(1 << 16)
+    call = lambda **kw: lib.hallo_rope(C.byref(_rope_desc(p, **kw)), None)
+    for origin in ((2 ** 31 - 1, 0), (0, 2 ** 31 - 2)):
+        assert call(origin=origin) == -22, origin
+    del keep
