@@ -351,7 +351,7 @@ extern "C" int hallo_layernorm_train(const void* x, int64_t ldx, void* y, int64_
   if (rows < 0 || C < 1 || C > LN_MAX_C || ldx < C || ldy < C || !(eps >= 0.0f) || (affine_f32 & ~1) || (dtype != DT_F16 && dtype != DT_BF16))
     return -22;
   if (rows == 0) return 0;
-  if (!x || !y || !stats) return -22;
+  if (!x || !y || !stats || (x == y && ldx != ldy && rows > 1)) return -22;
   hipStream_t st = (hipStream_t)stream;
   return dtype == DT_F16 ? launch_fwd<_Float16>(x, ldx, y, ldy, gamma, beta, affine_f32, stats, rows, C, eps, st)
                          : launch_fwd<__bf16>(x, ldx, y, ldy, gamma, beta, affine_f32, stats, rows, C, eps, st);
@@ -373,6 +373,7 @@ extern "C" int hallo_layernorm_backward(const void* dy, int64_t lddy, const void
     return -22;
   if ((dgamma == nullptr) != (dbeta == nullptr)) return -22;
   if (rows > 0 && (!dy || !x || !stats || !dx)) return -22;
+  if (rows > 1 && ((dx == dy && lddx != lddy) || (dx == x && lddx != ldx))) return -22;
   if (dgamma && rows > 0 && (!workspace || workspace_bytes < hallo_layernorm_backward_workspace(rows, C))) return -22;
   hipStream_t st = (hipStream_t)stream;
   return dtype == DT_F16

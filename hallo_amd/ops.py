@@ -8,6 +8,7 @@ import ctypes as C
 import math
 import threading
 
+import numpy as np
 import torch
 
 from . import lib as _l
@@ -887,6 +888,38 @@ def _like(name, t, like, dtype=None, shape=True):
         _bad(f"{name}: expected {tuple(like.shape)}, got {tuple(t.shape)}")
 
 
+class _Places:
+    """The memory of a strided tensor, for numpy's overlap test (nothing is read)."""
+
+    def __init__(self, t):
+        n = t.element_size()
+        self.__array_interface__ = {"data": (t.data_ptr(), False), "shape": tuple(t.shape), "strides": tuple(s * n for s in t.stride()),
+                                    "typestr": f"|V{n}", "version": 3}
+
+
+def _apart(name, out, others, same=()):
+    """`out` (given by the caller) shares no memory with `others`, nor with `same` unless it is the same view: rows are written while
+    other workgroups still read.  Column slices of one buffer are apart."""
+    if not out.numel():
+        return
+    dims = [(n, s) for n, s in zip(out.shape, out.stride()) if n > 1]
+    lo, hi = out.data_ptr(), out.data_ptr() + (1 + sum((n - 1) * s for n, s in dims)) * out.element_size()
+    for i, (other, t) in enumerate((*same, *others)):
+        if t is None or not t.numel():
+            continue
+        at = t.data_ptr()
+        if at >= hi or at + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() <= lo:
+            continue
+        if i < len(same) and at == lo and t.shape == out.shape and [(n, s) for n, s in zip(t.shape, t.stride()) if n > 1] == dims:
+            continue
+        try:
+            met = np.shares_memory(np.asarray(_Places(out)), np.asarray(_Places(t)), max_work=1 << 20)
+        except RuntimeError:                     # strides too odd to tell within that work
+            met = True
+        if met:
+            _bad(f"{name}: overlaps {other}")
+
+
 def _rows2d(name, x):
     """x [..., C] as (rows, C, row pitch): contiguous, or a 2-D view with contiguous rows."""
     sh = x.shape
@@ -914,7 +947,8 @@ def _affine(x, gamma, beta):
 
 def layernorm_train(x, gamma=None, beta=None, eps=1e-5, *, out=None):
     """(y, stats): y = LayerNorm(x [..., C]) * gamma + beta and the row statistics fp32 [rows, 2] = (mean, rstd) that
-    layernorm_backward() takes.  Any C up to 16384.  gamma / beta: [C] of x's type or fp32 (master weights), or None.  out may be x."""
+    layernorm_backward() takes.  Any C up to 16384.  gamma / beta: [C] of x's type or fp32 (master weights), or None.  out may be x, but not lie
+    on part of it."""
     _chk_dev(x, gamma, beta, out)
     code = dtype_code(x.dtype)
     rows, Cd, ldx = _rows2d("x", x)
@@ -923,6 +957,7 @@ def layernorm_train(x, gamma=None, beta=None, eps=1e-5, *, out=None):
         out = torch.empty_like(x)
     else:
         _like("out", out, x)
+        _apart("out", out, (("gamma", gamma), ("beta", beta)), (("x", x),))
     ldy = _rows2d("out", out)[2]
     stats = torch.empty((rows, 2), device=x.device, dtype=torch.float32)
     _call("hallo_layernorm_train", x.device, x.data_ptr(), ldx, out.data_ptr(), ldy, gamma.data_ptr() if gamma is not None else None,
@@ -946,6 +981,7 @@ def layernorm_backward(dy, x, stats, gamma=None, *, weight_grads=True, out=None)
         out = torch.empty_like(x)
     else:
         _like("out", out, x)
+        _apart("out", out, (("stats", stats), ("gamma", gamma)), (("dy", dy), ("x", x)))
     ldo = _rows2d("out", out)[2]
     dg = db = pg = pb = pw = None
     need = 0
@@ -1000,7 +1036,8 @@ def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
     """Rotary positions on x [B, L, heads * head_dim] (any batch / row stride: column slices of a fused q|k|v buffer, q|k together).
 
     Positions: pos int32 [L, axes] or [B, L, axes]; or grid = the axes' lengths with L cells, the last axis fastest, counted from
-    `origin` (default 0).  inverse=True turns back: the gradient with respect to x of rope(x) is rope(dy, inverse=True).  out may be x."""
+    `origin` (default 0).  inverse=True turns back: the gradient with respect to x of rope(x) is rope(dy, inverse=True).  out may be x, but
+    not lie on part of it."""
     _chk_dev(x, pos, out, axes.freq)
     code = dtype_code(x.dtype)
     n, hd, sh, st = len(axes.dims), axes.head_dim, x.shape, x.stride()
@@ -1009,7 +1046,8 @@ def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
     if axes.freq.device != x.device:
         _bad(f"axes were built on {axes.freq.device}, x is on {x.device}")
     B, L, W = sh
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(x)
     else:
         _like("out", out, x)
@@ -1018,6 +1056,8 @@ def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
     so = out.stride()
     if so[2] != 1 or (L > 1 and so[1] < W) or (B > 1 and L and _entries_meet(B, L, so[0], so[1], W)):
         _bad(f"out: expected {tuple(sh)} with rows that do not overlap, got {tuple(out.shape)} strides {so}")
+    if given:
+        _apart("out", out, (("pos", pos), ("the frequencies", axes.freq)), (("x", x),))
     if (pos is None) == (grid is None):
         _bad("give either pos or grid")
     pp, pbs = None, 0
@@ -1141,6 +1181,8 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
         _like("out", out, q)
     lse = torch.empty((q.shape[0], heads, q.shape[1]), device=q.device, dtype=torch.float32) if return_lse and heads >= 1 else None
     d, _, _ = _window_desc(q, k, v, out, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, given)
+    if given:
+        _apart("out", out, (("q", q), ("k", k), ("v", v), ("q_len", q_len), ("kv_len", kv_len)))
     need = _l.load().hallo_window_attention_workspace(C.byref(d))
     if need:
         if need < 0:
@@ -1154,7 +1196,7 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
 def window_attention_backward(do, q, k, v, o, lse, heads, *, kv_heads=None, left=-1, right=0, sinks=0, q_len=None, kv_len=None, scale=None,
                               dq=None, dk=None, dv=None):
     """(dq, dk, dv) of o, lse = window_attention(q, k, v, ..., return_lse=True) for do, with the same arguments.  dk / dv are summed over
-    the query heads that share a key head; padded rows get zeros.  dq / dk / dv must not overlap the inputs.  Results repeat bit for bit."""
+    the query heads that share a key head; padded rows get zeros.  dq / dk / dv must overlap neither the inputs nor one another.  Results repeat bit for bit."""
     _chk_dev(do, q, k, v, o, lse, q_len, kv_len, dq, dk, dv)
     _like("o", o, q)
     _like("do", do, q)
@@ -1171,6 +1213,13 @@ def window_attention_backward(do, q, k, v, o, lse, heads, *, kv_heads=None, left
             t = torch.empty(like.shape, device=q.device, dtype=q.dtype)
         outs.append(t)
         strides += _heads4(name, t, n, hd, given)
+    inputs = ("do", do), ("q", q), ("k", k), ("v", v), ("o", o), ("lse", lse), ("q_len", q_len), ("kv_len", kv_len)
+    if dq is not None:
+        _apart("dq", dq, (*inputs, ("dk", dk), ("dv", dv)))
+    if dk is not None:
+        _apart("dk", dk, (*inputs, ("dv", dv)))
+    if dv is not None:
+        _apart("dv", dv, inputs)
     dq, dk, dv = outs
     d = _l.WindowAttnBwdDesc(w, do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *_heads4("do", do, heads, hd), *strides)
     need = _l.load().hallo_window_attention_backward_workspace(C.byref(d))

@@ -426,11 +426,11 @@ int hallo_lerp_rows(const void* x, void* y, int in_rows, int out_rows, int C, in
  * (The entry points from here on came without a new version number: nothing before them changed.)
  * LayerNorm for training.  x [rows, C] (row pitch ldx >= C elements, any C in 1 .. 16384, any alignment), stats fp32 [rows][2] =
  * (mean, rstd).  gamma / beta [C] in `dtype`, or fp32 with affine_f32 = 1; null = 1 / 0.
- * hallo_layernorm_train:    y = (x - mean) * rstd * gamma + beta, and stats.  y may be x.
+ * hallo_layernorm_train:    y = (x - mean) * rstd * gamma + beta, and stats.  y may be x (same pitch; else they must not overlap).
  * hallo_layernorm_backward: with xh = (x - mean) * rstd and g = dy * gamma
  *   dx = rstd * (g - mean_C(g) - xh * mean_C(g * xh)),  dgamma[c] = sum_rows(dy * xh),  dbeta[c] = sum_rows(dy)
- *   dgamma / dbeta are fp32 [C]; both null: only dx.  dx may be dy.  workspace: hallo_layernorm_backward_workspace(rows, C) bytes
- *   (needed with dgamma).  Sums run in a fixed order: results repeat bit for bit.
+ *   dgamma / dbeta are fp32 [C]; both null: only dx.  dx may be dy or x (same pitch; else it must not overlap the inputs).
+ *   workspace: hallo_layernorm_backward_workspace(rows, C) bytes (needed with dgamma).  Sums run in a fixed order: results repeat bit for bit.
  */
 int hallo_layernorm_train(const void* x, int64_t ldx, void* y, int64_t ldy, const void* gamma, const void* beta, int affine_f32,
                           float* stats, int64_t rows, int C, float eps, int dtype, void* stream);

@@ -50,3 +50,84 @@ def test_rope_abi_positions_past_32_bits(lib):  # noqa: F811
     for origin in ((2 ** 31 - 1, 0), (0, 2 ** 31 - 2)):
         assert call(origin=origin) == -22, origin
     del keep
+
+
+def _accepted(f, *a, **kw):
+    f(*a, **kw)
+
+
+def _refused(f, *a, match, **kw):
+    with pytest.raises(Err, match=match):
+        f(*a, **kw)
+
+
+def test_layernorm_outputs_on_inputs(host):  # noqa: F811
+    host.setattr(ops, "_call", lambda *a: None)
+    buf = torch.zeros(4096, dtype=H)
+    rows = lambda off, pitch=48, n=8: buf.as_strided((n, 32), (pitch, 1), off)
+    x, gamma, stats = rows(0), buf[3000:3032], torch.zeros(8, 2)
+    far = buf[2000:2256].view(8, 32)
+    for out in (rows(8), rows(48), rows(0, 64), rows(0, 32), rows(24, 96)):
+        _refused(ops.layernorm_train, x, out=out, match="overlaps x")
+        _refused(ops.layernorm_backward, far, x, stats, out=out, weight_grads=False, match="overlaps x")
+        _refused(ops.layernorm_backward, x, far, stats, out=out, weight_grads=False, match="overlaps dy")
+    _refused(ops.layernorm_train, x, gamma, out=rows(2900), match="overlaps gamma")
+    _refused(ops.layernorm_train, x, None, gamma, out=rows(2900), match="overlaps beta")
+    wide = buf.as_strided((8, 32), (96, 1), 0)
+    for out in (rows(0), far, rows(8 * 48)):     # the same rows, others, behind them
+        _accepted(ops.layernorm_train, x, out=out)
+        _accepted(ops.layernorm_backward, far, x, stats, out=out, weight_grads=False)
+    for off in (32, 64):                         # column slices of one buffer
+        _accepted(ops.layernorm_train, wide, out=buf.as_strided((8, 32), (96, 1), off))
+    one = buf.as_strided((1, 32), (7, 1), 0)     # the stride of a single row does not count
+    _accepted(ops.layernorm_train, buf.as_strided((1, 32), (32, 1), 0), out=one)
+
+
+def test_layernorm_abi_in_place_at_another_pitch(lib):  # noqa: F811
+    keep, p = _mem(1 << 16)
+    q = p + 8192
+    assert lib.hallo_layernorm_train(p, 32, p, 40, None, None, 0, q, 4, 32, 1e-5, 0, None) == -22
+    for dy, x, lddy, ldx in ((p, q, 32, 40), (q, p, 40, 32)):
+        assert lib.hallo_layernorm_backward(dy, lddy, x, ldx, q, None, 0, p, 40, None, None, None, 0, 4, 32, 0, None) == -22
+    del keep
+
+
+def test_rope_outputs_on_inputs(host):  # noqa: F811
+    host.setattr(ops, "_call", lambda *a: None)
+    axes = ops.RopeAxes((8, 8), 16, device="cpu")
+    buf = torch.zeros(8192, dtype=H)
+    at = lambda off, bs=600, rs=96: buf.as_strided((2, 6, 32), (bs, rs, 1), off)
+    x, pos = at(0), torch.zeros(6, 2, dtype=torch.int32)
+    for out in (at(8), at(96), at(0, 600, 64), at(0, 700), at(80)):
+        _refused(ops.rope, x, axes, pos=pos, out=out, match="overlaps x")
+    for out in (at(0), at(32), at(64), at(2000)):
+        _accepted(ops.rope, x, axes, pos=pos, out=out)
+
+
+def test_window_attention_outputs_on_inputs(host):  # noqa: F811
+    host.setattr(ops, "_call", lambda *a: None)
+
+    class Lib:
+        hallo_window_attention_workspace = hallo_window_attention_backward_workspace = staticmethod(lambda d: 0)
+    host.setattr(ops._l, "load", lambda *a: Lib)
+    q, k, v = (torch.zeros(2, 5, 64, dtype=H) for _ in range(3))
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _refused(ops.window_attention, q, k, v, 4, out=t, match=f"overlaps {name}")
+    fused = torch.zeros(2, 5, 256, dtype=H)
+    parts = fused.split(64, 2)
+    _accepted(ops.window_attention, *parts[:3], 4, out=parts[3])
+    _refused(ops.window_attention, *parts[:3], 4, out=fused[..., 184:248], match="overlaps v")
+    heads = torch.zeros(2, 8, 5, 16, dtype=H)    # head-major
+    _accepted(ops.window_attention, q.view(2, 5, 4, 16), k, v, 4, out=heads[:, 4:].transpose(1, 2))
+    _refused(ops.window_attention, heads[:, :4].transpose(1, 2), k, v, 4, out=heads[:, 3:7].transpose(1, 2), match="overlaps q")
+    lse, do, o = torch.zeros(2, 4, 5), torch.zeros_like(q), torch.zeros_like(q)
+    b = lambda **kw: ops.window_attention_backward(do, q, k, v, o, lse, 4, **kw)
+    for name, t in (("do", do), ("q", q), ("k", k), ("v", v), ("o", o)):
+        for out in ("dq", "dk", "dv"):
+            _refused(b, **{out: t}, match=f"{out}: overlaps {name}")
+    d = torch.zeros_like(q)
+    for a, c in (("dq", "dk"), ("dq", "dv"), ("dk", "dv")):
+        _refused(b, **{a: d, c: d}, match=f"{a}: overlaps {c}")
+        _refused(b, **{a: fused[..., :64], c: fused[..., 32:96]}, match=f"{a}: overlaps {c}")
+    _accepted(b, dq=parts[0], dk=parts[1], dv=parts[2])
+    _accepted(b, dq=parts[0])
