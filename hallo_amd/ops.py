@@ -857,8 +857,9 @@ def lerp_rows(x, out_rows):
 
 # ---- transformer-block operators with gradients: LayerNorm, rotary positions, window attention -------------------------------------
 # Their workspaces are allocated per call: a captured graph gets them from its own pool, so two graphs never share one, and the
-# allocator orders the reuse of a freed one on its stream.  Single tokens and short rows are host-bound, so messages are only put
-# together where a call is refused.
+# allocator orders the reuse of a freed one on its stream.  They are not torch functions with a gradient: forward and backward are calls
+# of their own, and a forward call refuses tensors that wait for a gradient (where torch records).  Single tokens and short rows are
+# host-bound, so messages are only put together where a call is refused.
 
 def _bad(what):
     raise _l.HalloLibraryError(what)
@@ -876,6 +877,14 @@ def _call(name, device, *args):
             status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     if status:
         _l.check(status, name)
+
+
+def _no_graph(*tensors):
+    """The forward calls record nothing for torch's differentiation: refused where torch records and a tensor takes part in it."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            _bad(f"a tensor of shape {tuple(t.shape)} needs a gradient, which this call does not record: call it under torch.no_grad() or in an "
+                 "autograd.Function, and its backward operator for the gradients")
 
 
 def _like(name, t, like, dtype=None, shape=True):
@@ -950,6 +959,7 @@ def layernorm_train(x, gamma=None, beta=None, eps=1e-5, *, out=None):
     layernorm_backward() takes.  Any C up to 16384.  gamma / beta: [C] of x's type or fp32 (master weights), or None.  out may be x, but not lie
     on part of it."""
     _chk_dev(x, gamma, beta, out)
+    _no_graph(x, gamma, beta, out)
     code = dtype_code(x.dtype)
     rows, Cd, ldx = _rows2d("x", x)
     f32 = _affine(x, gamma, beta)
@@ -1039,6 +1049,7 @@ def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
     `origin` (default 0).  inverse=True turns back: the gradient with respect to x of rope(x) is rope(dy, inverse=True).  out may be x, but
     not lie on part of it."""
     _chk_dev(x, pos, out, axes.freq)
+    _no_graph(x, out)
     code = dtype_code(x.dtype)
     n, hd, sh, st = len(axes.dims), axes.head_dim, x.shape, x.stride()
     if len(sh) != 3 or sh[2] % hd or not sh[2] or st[2] != 1:
@@ -1174,6 +1185,7 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
 
     return_lse: (out, lse), lse fp32 [B, heads, Lq] (-inf where nothing is visible), as window_attention_backward() takes it."""
     _chk_dev(q, k, v, q_len, kv_len, out)
+    _no_graph(q, k, v, out)
     given = out is not None
     if not given:
         out = torch.empty_like(q)

@@ -131,3 +131,48 @@ def test_window_attention_outputs_on_inputs(host):  # noqa: F811
         _refused(b, **{a: fused[..., :64], c: fused[..., 32:96]}, match=f"{a}: overlaps {c}")
     _accepted(b, dq=parts[0], dk=parts[1], dv=parts[2])
     _accepted(b, dq=parts[0])
+
+
+def test_inputs_that_need_a_gradient(host):  # noqa: F811
+    """The forward calls record nothing for torch's differentiation: an input that waits for a gradient would silently get none."""
+    host.setattr(ops, "_call", lambda *a: None)
+
+    class Lib:
+        hallo_window_attention_workspace = staticmethod(lambda d: 0)
+    host.setattr(ops._l, "load", lambda *a: Lib)
+    leaf = lambda *s: torch.zeros(*s, dtype=H, requires_grad=True)
+    x, w, axes = torch.zeros(4, 32, dtype=H), torch.zeros(32, dtype=H), ops.RopeAxes((8, 8), 16, device="cpu")
+    s, pos = torch.zeros(2, 6, 32, dtype=H), torch.zeros(6, 2, dtype=torch.int32)
+    calls = [(ops.layernorm_train, (leaf(4, 32),), {}), (ops.layernorm_train, (x, leaf(32), w), {}), (ops.layernorm_train, (x, w, leaf(32)), {}),
+             (ops.layernorm_train, (x, torch.ones(32, requires_grad=True)), {}), (ops.rope, (leaf(2, 6, 32), axes), dict(pos=pos)),
+             (ops.window_attention, (leaf(2, 6, 32), s, s, 2), {}), (ops.window_attention, (s, leaf(2, 6, 32), s, 2), {}),
+             (ops.window_attention, (s, s, leaf(2, 6, 32) * 1, 2), {}), (ops.layernorm_train, (x,), dict(out=leaf(4, 32))),
+             (ops.rope, (s, axes), dict(pos=pos, out=leaf(2, 6, 32))), (ops.window_attention, (s, s, s, 2), dict(out=leaf(2, 6, 32)))]
+    for f, a, kw in calls:
+        _refused(f, *a, **kw, match="gradient")
+        with torch.no_grad():
+            _accepted(f, *a, **kw)
+        with torch.inference_mode():
+            _accepted(f, *a, **kw)
+        cut = lambda t: t.detach() if torch.is_tensor(t) else t
+        _accepted(f, *map(cut, a), **{n: cut(t) for n, t in kw.items()})
+
+
+def test_inside_a_function_of_torch(host):  # noqa: F811
+    """torch calls forward() of an autograd.Function without recording: the calls a user's own Function makes pass."""
+    host.setattr(ops, "_call", lambda *a: None)
+
+    class Norm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, gamma):
+            y, stats = ops.layernorm_train(x, gamma)
+            ctx.save_for_backward(x, gamma, stats)
+            return y
+
+        @staticmethod
+        def backward(ctx, dy):
+            x, gamma, stats = ctx.saved_tensors
+            return ops.layernorm_backward(dy.contiguous(), x, stats, gamma, weight_grads=False)[0], None
+    x = torch.zeros(4, 32, dtype=H, requires_grad=True)
+    Norm.apply(x, torch.ones(32, dtype=H)).sum().backward()
+    assert x.grad.shape == x.shape
