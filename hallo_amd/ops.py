@@ -887,6 +887,13 @@ def _no_graph(*tensors):
                  "autograd.Function, and its backward operator for the gradients")
 
 
+def _written(*tensors):
+    """Outputs that the caller gave: torch counts the call as a change of them (what it keeps for a gradient is then known to be stale)."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _like(name, t, like, dtype=None, shape=True):
     """`t` is on `like`'s device, of its type (or `dtype`) and, with `shape`, of its shape."""
     if t.device != like.device:
@@ -963,7 +970,8 @@ def layernorm_train(x, gamma=None, beta=None, eps=1e-5, *, out=None):
     code = dtype_code(x.dtype)
     rows, Cd, ldx = _rows2d("x", x)
     f32 = _affine(x, gamma, beta)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(x)
     else:
         _like("out", out, x)
@@ -972,6 +980,8 @@ def layernorm_train(x, gamma=None, beta=None, eps=1e-5, *, out=None):
     stats = torch.empty((rows, 2), device=x.device, dtype=torch.float32)
     _call("hallo_layernorm_train", x.device, x.data_ptr(), ldx, out.data_ptr(), ldy, gamma.data_ptr() if gamma is not None else None,
           beta.data_ptr() if beta is not None else None, f32, stats.data_ptr(), rows, Cd, float(eps), code)
+    if given:
+        _written(out)
     return out, stats
 
 
@@ -987,7 +997,8 @@ def layernorm_backward(dy, x, stats, gamma=None, *, weight_grads=True, out=None)
     if stats.shape != (rows, 2) or not stats.is_contiguous():
         _bad(f"stats: expected contiguous ({rows}, 2), got {tuple(stats.shape)}")
     f32 = _affine(x, gamma, None)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(x)
     else:
         _like("out", out, x)
@@ -1006,6 +1017,8 @@ def layernorm_backward(dy, x, stats, gamma=None, *, weight_grads=True, out=None)
         pb, pw = pg + 4 * Cd, ws.data_ptr()
     _call("hallo_layernorm_backward", x.device, dy.data_ptr(), ldd, x.data_ptr(), ldx, stats.data_ptr(),
           gamma.data_ptr() if gamma is not None else None, f32, out.data_ptr(), ldo, pg, pb, pw, need, rows, Cd, code)
+    if given:
+        _written(out)
     return out, dg, db
 
 
@@ -1093,6 +1106,8 @@ def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
     d = _l.RopeDesc(x.data_ptr(), out.data_ptr(), st[0] if B > 1 else 0, st[1] if L > 1 else W, so[0] if B > 1 else 0, so[1] if L > 1 else W,
                     axes.freq.data_ptr(), pp, pbs, B, L, W // hd, hd, n, axes.dims, grid, origin, axes.interleaved, bool(inverse), code)
     _call("hallo_rope", x.device, C.byref(d))
+    if given:
+        _written(out)
     return out
 
 
@@ -1202,6 +1217,8 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
         ws = torch.empty(need // 4, device=q.device, dtype=torch.float32)
         d.workspace, d.workspace_bytes = ws.data_ptr(), need
     _call("hallo_window_attention", q.device, C.byref(d))
+    if given:
+        _written(out)
     return (out, lse) if return_lse else out
 
 
@@ -1232,7 +1249,7 @@ def window_attention_backward(do, q, k, v, o, lse, heads, *, kv_heads=None, left
         _apart("dk", dk, (*inputs, ("dv", dv)))
     if dv is not None:
         _apart("dv", dv, inputs)
-    dq, dk, dv = outs
+    given, (dq, dk, dv) = (dq, dk, dv), outs
     d = _l.WindowAttnBwdDesc(w, do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *_heads4("do", do, heads, hd), *strides)
     need = _l.load().hallo_window_attention_backward_workspace(C.byref(d))
     if need < 0:
@@ -1240,4 +1257,5 @@ def window_attention_backward(do, q, k, v, o, lse, heads, *, kv_heads=None, left
     ws = torch.empty(max(need // 4, 4), device=q.device, dtype=torch.float32)
     d.fwd.workspace, d.fwd.workspace_bytes = ws.data_ptr(), need
     _call("hallo_window_attention_backward", q.device, C.byref(d))
+    _written(*given)
     return dq, dk, dv

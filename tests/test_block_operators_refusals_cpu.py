@@ -176,3 +176,28 @@ def test_inside_a_function_of_torch(host):  # noqa: F811
     x = torch.zeros(4, 32, dtype=H, requires_grad=True)
     Norm.apply(x, torch.ones(32, dtype=H)).sum().backward()
     assert x.grad.shape == x.shape
+
+
+def test_given_outputs_count_as_changed(host):  # noqa: F811
+    """torch notices that a tensor which it keeps for a gradient was written: its version goes up with every call that is given it."""
+    host.setattr(ops, "_call", lambda *a: None)
+
+    class Lib:
+        hallo_window_attention_workspace = hallo_window_attention_backward_workspace = staticmethod(lambda d: 0)
+    host.setattr(ops._l, "load", lambda *a: Lib)
+    x, stats, axes, pos = torch.zeros(2, 6, 32, dtype=H), torch.zeros(12, 2), ops.RopeAxes((8, 8), 16, device="cpu"), torch.zeros(6, 2, dtype=torch.int32)
+    a = [torch.zeros_like(x) for _ in range(6)]
+    lse, new = torch.zeros(2, 2, 6), lambda: torch.zeros_like(x)
+    calls = [lambda t: ops.layernorm_train(x, out=t), lambda t: ops.layernorm_backward(x, x, stats, weight_grads=False, out=t),
+             lambda t: ops.rope(x, axes, pos=pos, out=t), lambda t: ops.window_attention(*a[:3], 2, out=t)]
+    calls += [lambda t, n=n: ops.window_attention_backward(*a[:5], lse, 2, **{n: t}) for n in ("dq", "dk", "dv")]
+    for f in calls:
+        t, w = new(), torch.zeros(2, 6, 32, dtype=H, requires_grad=True)
+        kept = (w * t).sum()
+        v = t._version
+        f(t)
+        assert t._version > v
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.backward()
+        with torch.inference_mode():
+            f(new())
