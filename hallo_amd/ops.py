@@ -1206,7 +1206,9 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
         out = torch.empty_like(q)
     else:
         _like("out", out, q)
-    lse = torch.empty((q.shape[0], heads, q.shape[1]), device=q.device, dtype=torch.float32) if return_lse and heads >= 1 else None
+    lse = None
+    if return_lse and heads >= 1 and q.dim() > 2:
+        lse = torch.empty((q.shape[0], heads, q.shape[1]), device=q.device, dtype=torch.float32)
     d, _, _ = _window_desc(q, k, v, out, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, given)
     if given:
         _apart("out", out, (("q", q), ("k", k), ("v", v), ("q_len", q_len), ("kv_len", kv_len)))
@@ -1230,6 +1232,8 @@ def window_attention_backward(do, q, k, v, o, lse, heads, *, kv_heads=None, left
     _like("o", o, q)
     _like("do", do, q)
     _like("lse", lse, q, torch.float32, False)
+    if q.dim() < 3:
+        _bad(f"q: expected [B, L, {heads} * head_dim] or [B, L, {heads}, head_dim], got {tuple(q.shape)}")
     if lse.shape != (q.shape[0], heads, q.shape[1]) or not lse.is_contiguous():
         _bad(f"lse: expected contiguous ({q.shape[0]}, {heads}, {q.shape[1]}), got {tuple(lse.shape)}")
     w, kv_heads, hd = _window_desc(q, k, v, o, lse, heads, kv_heads, left, right, sinks, q_len, kv_len, scale, False)

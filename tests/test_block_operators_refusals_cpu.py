@@ -201,3 +201,10 @@ def test_given_outputs_count_as_changed(host):  # noqa: F811
             kept.backward()
         with torch.inference_mode():
             f(new())
+
+
+def test_tensors_of_one_dimension(host):  # noqa: F811
+    q, one, lse = torch.zeros(2, 5, 64, dtype=H), torch.zeros(64, dtype=H), torch.zeros(2, 2, 5)
+    for lse_too in (False, True):
+        _refused(ops.window_attention, one, q, q, 2, return_lse=lse_too, match="q:")
+    _refused(ops.window_attention_backward, one, one, q, q, one, lse, 2, match="q:")
