@@ -1036,7 +1036,10 @@ class RopeAxes:
         if not theta > 0 or not math.isfinite(theta):
             _bad(f"theta: expected a positive number, got {theta}")
         self.dims, self.head_dim, self.theta, self.interleaved = dims, int(head_dim), float(theta), bool(interleaved)
-        turns = [int(round(self.theta ** (-2.0 * i / d) / (2.0 * math.pi) * 2.0 ** 64)) % (1 << 64) for d in dims for i in range(d // 2)]
+        try:
+            turns = [int(round(self.theta ** (-2.0 * i / d) / (2.0 * math.pi) * 2.0 ** 64)) % (1 << 64) for d in dims for i in range(d // 2)]
+        except OverflowError:
+            _bad(f"theta {theta}: its frequencies pass the range of a float")
         self.freq = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64).to(device)
 
 

@@ -208,3 +208,8 @@ def test_tensors_of_one_dimension(host):  # noqa: F811
     for lse_too in (False, True):
         _refused(ops.window_attention, one, q, q, 2, return_lse=lse_too, match="q:")
     _refused(ops.window_attention_backward, one, one, q, q, one, lse, 2, match="q:")
+
+
+def test_rope_frequencies_past_a_float():
+    for theta in (1e-300, 5e-324):
+        _refused(ops.RopeAxes, (64,), 64, theta=theta, device="cpu", match="theta")
