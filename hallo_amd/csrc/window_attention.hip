@@ -567,6 +567,15 @@ extern "C" int64_t hallo_window_attention_workspace(const hallo_window_attn_desc
   return a.nsplit > 1 ? (int64_t)a.batch * a.kv_heads * a.nrb * a.nsplit * 32 * (a.hd + 2) * 4 : 0;
 }
 
+extern "C" int hallo_window_attention_splits(const hallo_window_attn_desc* d) {
+  using namespace hallo;
+  WinArgs a;
+  if (!win_args(d, a)) return -22;
+  if (a.batch == 0 || a.Lq == 0) return 0;
+  plan(a);
+  return a.nsplit;
+}
+
 extern "C" int hallo_window_attention(const hallo_window_attn_desc* d, void* stream) {
   using namespace hallo;
   WinArgs a;

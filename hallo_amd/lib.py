@@ -191,6 +191,7 @@ SYMBOLS = {
                                            C.c_void_p]),
     "hallo_rope": (C.c_int, [C.POINTER(RopeDesc), C.c_void_p]),
     "hallo_window_attention_workspace": (C.c_int64, [C.POINTER(WindowAttnDesc)]),
+    "hallo_window_attention_splits": (C.c_int, [C.POINTER(WindowAttnDesc)]),
     "hallo_window_attention": (C.c_int, [C.POINTER(WindowAttnDesc), C.c_void_p]),
     "hallo_window_attention_backward_workspace": (C.c_int64, [C.POINTER(WindowAttnBwdDesc)]),
     "hallo_window_attention_backward": (C.c_int, [C.POINTER(WindowAttnBwdDesc), C.c_void_p]),

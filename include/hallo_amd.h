@@ -473,6 +473,9 @@ int hallo_rope(const hallo_rope_desc* d, void* stream);
  * What lies at or behind kv_len, or outside of every query's window, is not used and may hold anything.
  * workspace: hallo_window_attention_workspace(d) bytes, 0 unless the keys are split over workgroups.
  *
+ * hallo_window_attention_splits: the way a call is divided, without making it: 0 = blocks of 128 queries, n > 0 = packed blocks of 32 query
+ * rows with the keys in n parts (decided on the host, from the descriptor alone).
+ *
  * hallo_window_attention_backward: dq, dk, dv for dout, with q, k, v, o, lse and the mask as in `fwd` (fwd.o and fwd.lse are read; lse
  * must be there).  dk / dv are summed over the query heads of a key head; rows at or behind q_len / kv_len are written as zeros.
  * dq, dk, dv must overlap neither the inputs nor one another.  Deterministic.  fwd.workspace: hallo_window_attention_backward_workspace(d) bytes.
@@ -496,6 +499,7 @@ typedef struct hallo_window_attn_bwd_desc {
   int64_t do_bs, do_rs, do_hs, dq_bs, dq_rs, dq_hs, dk_bs, dk_rs, dk_hs, dv_bs, dv_rs, dv_hs;
 } hallo_window_attn_bwd_desc;
 int64_t hallo_window_attention_workspace(const hallo_window_attn_desc* d);
+int hallo_window_attention_splits(const hallo_window_attn_desc* d);
 int hallo_window_attention(const hallo_window_attn_desc* d, void* stream);
 int64_t hallo_window_attention_backward_workspace(const hallo_window_attn_bwd_desc* d);
 int hallo_window_attention_backward(const hallo_window_attn_bwd_desc* d, void* stream);

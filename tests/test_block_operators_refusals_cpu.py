@@ -213,3 +213,14 @@ def test_tensors_of_one_dimension(host):  # noqa: F811
 def test_rope_frequencies_past_a_float():
     for theta in (1e-300, 5e-324):
         _refused(ops.RopeAxes, (64,), 64, theta=theta, device="cpu", match="theta")
+
+
+def test_window_attention_splits(lib):  # noqa: F811
+    """How a call is divided, from its descriptor alone: one form refuses what the call refuses, and needs no memory."""
+    from test_block_operators_cpu import BAD_ATTN, _attn_desc
+    ask = lambda **kw: lib.hallo_window_attention_splits(C.byref(_attn_desc(0, **kw)))
+    assert lib.hallo_window_attention_splits(None) == -22
+    for kw in BAD_ATTN:
+        assert ask(**kw) == -22, kw
+    assert ask(batch=0) == 0 and ask(Lq=0) == 0 and ask() == 1
+    assert ask(Lq=1, Lk=100000, left=-1) > 1 and ask(batch=64, heads=32, kv_heads=32, Lq=1000, Lk=1000) == 0
