@@ -35,6 +35,20 @@ def _stale(out, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _flags(cmd):
+    """Of a compile command, what decides about the object besides the sources."""
+    return " ".join(cmd[1:cmd.index("-c")])
+
+
+def _built_with(o):
+    """The flags that an object was built with: other ones make it stale as a newer source does."""
+    try:
+        with open(o + ".flags") as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def build(force=False, verbose=False):
     """Compile every HIP source for gfx950 and link libhallo_amd.so.  Returns the library path."""
     hipcc = _hipcc()
@@ -44,10 +58,10 @@ def build(force=False, verbose=False):
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(objdir, src.replace(".hip", ".o"))
-        if force or _stale(o, [s] + HEADERS):
-            cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", *NO_PACKED_FP32, "-c", s, "-o", o]
-            if os.environ.get("HALLO_ABLATIONS") == "1":      # timing-ablation switches of the row-stationary GEMMs (tools/cbench)
-                cmd.insert(1, "-DHALLO_ABLATIONS")
+        cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", *NO_PACKED_FP32, "-c", s, "-o", o]
+        if os.environ.get("HALLO_ABLATIONS") == "1":      # timing-ablation switches of the row-stationary GEMMs (tools/cbench)
+            cmd.insert(1, "-DHALLO_ABLATIONS")
+        if force or _stale(o, [s] + HEADERS) or _built_with(o) != _flags(cmd):
             todo.append(cmd)
         objs.append(o)
 
@@ -55,6 +69,8 @@ def build(force=False, verbose=False):
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)
+        with open(cmd[-1] + ".flags", "w") as f:
+            f.write(_flags(cmd))
 
     with ThreadPoolExecutor(min(8, int(os.environ.get("MAX_JOBS") or 8), max(len(todo), 1))) as pool:
         list(pool.map(compile_one, todo))
