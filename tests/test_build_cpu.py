@@ -63,3 +63,15 @@ def test_other_flags(tree):
     assert built()[:2] == ["a.o", "b.o"]
     m.delenv("HALLO_ABLATIONS")
     assert built()[:2] == ["a.o", "b.o"]
+
+
+def test_every_compile_line_leaves_packed_fp32_out():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    flags, lines = " ".join(b.NO_PACKED_FP32), []
+    for top in ("hallo_amd", "tools"):
+        for folder, _, files in os.walk(os.path.join(root, top)):
+            for n in files:
+                if n.endswith((".sh", ".hip", ".h")):
+                    with open(os.path.join(folder, n), errors="replace") as f:
+                        lines += [(n, line) for line in f if "hipcc" in line and "--offload-arch" in line]
+    assert len(lines) >= 4 and all(flags in line for _, line in lines), lines

@@ -2,7 +2,7 @@
 //   mode 0: buffer_load_dwordx4 ... lds   (LDS-DMA, 1 KiB per wave instruction, what the GEMM loaders use)
 //   mode 1: global_load_dwordx4 into VGPRs (register staging)
 // Each workgroup loops over a private 64 KiB window of a small (L2-resident) buffer, UNROLL loads in flight per wave.
-// Build: hipcc --offload-arch=gfx950 -O3 tools/microbench/fill_bench.hip -o /tmp/fill_bench ; run on the MI355X box.
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/microbench/fill_bench.hip -o /tmp/fill_bench ; run on the MI355X box.
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdlib.h>

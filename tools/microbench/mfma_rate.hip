@@ -1,7 +1,7 @@
 // MFMA issue-rate microbenchmark: v_mfma_f32_32x32x16_bf16 from registers only (no LDS, no memory), NACC independent
 // accumulators in rotation, operands random bf16, 1 or 2 waves per SIMD.  Prints achieved TFLOP/s and cycles per MFMA per SIMD
 // at the clock the chip sustains under this load.
-//   hipcc --offload-arch=gfx950 -O3 -o mfma_rate mfma_rate.hip && ./mfma_rate
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o mfma_rate mfma_rate.hip && ./mfma_rate
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdlib.h>

@@ -1,7 +1,7 @@
 // VALU issue-rate microbenchmark for gfx950: cycles per wave-instruction of v_exp_f32 / v_rcp_f32 / v_fma_f32 / v_cvt_pk_bf16_f32 /
 // v_max3_f32, alone and next to MFMAs of another accumulator, with 1, 2 and 3 waves per SIMD.  Backs the roofline argument
 // for the head-dim-40 attention (32 exponentials per lane per 64-key tile against 14 MFMAs) in DESIGN.md.
-//   hipcc --offload-arch=gfx950 -O3 valu_rate.hip -o valu_rate && ./valu_rate
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops valu_rate.hip -o valu_rate && ./valu_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
