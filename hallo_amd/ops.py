@@ -880,11 +880,10 @@ def _call(name, device, *args):
 
 
 def _no_graph(*tensors):
-    """The forward calls record nothing for torch's differentiation: refused where torch records and a tensor takes part in it."""
-    for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            _bad(f"a tensor of shape {tuple(t.shape)} needs a gradient, which this call does not record: call it under torch.no_grad() or in an "
-                 "autograd.Function, and its backward operator for the gradients")
+    """The forward calls record nothing for torch's differentiation: refused where torch records and one of `tensors` takes part in it."""
+    if torch.is_grad_enabled():
+        _bad(f"a tensor of shape {next(tuple(t.shape) for t in tensors if t is not None and t.requires_grad)} needs a gradient, which this "
+             "call does not record: call it under torch.no_grad() or in an autograd.Function, and its backward operator for the gradients")
 
 
 def _written(*tensors):
@@ -966,7 +965,8 @@ def layernorm_train(x, gamma=None, beta=None, eps=1e-5, *, out=None):
     layernorm_backward() takes.  Any C up to 16384.  gamma / beta: [C] of x's type or fp32 (master weights), or None.  out may be x, but not lie
     on part of it."""
     _chk_dev(x, gamma, beta, out)
-    _no_graph(x, gamma, beta, out)
+    if x.requires_grad or gamma is not None and gamma.requires_grad or beta is not None and beta.requires_grad or out is not None and out.requires_grad:
+        _no_graph(x, gamma, beta, out)
     code = dtype_code(x.dtype)
     rows, Cd, ldx = _rows2d("x", x)
     f32 = _affine(x, gamma, beta)
@@ -1065,7 +1065,8 @@ def rope(x, axes, *, grid=None, origin=None, pos=None, inverse=False, out=None):
     `origin` (default 0).  inverse=True turns back: the gradient with respect to x of rope(x) is rope(dy, inverse=True).  out may be x, but
     not lie on part of it."""
     _chk_dev(x, pos, out, axes.freq)
-    _no_graph(x, out)
+    if x.requires_grad or out is not None and out.requires_grad:
+        _no_graph(x, out)
     code = dtype_code(x.dtype)
     n, hd, sh, st = len(axes.dims), axes.head_dim, x.shape, x.stride()
     if len(sh) != 3 or sh[2] % hd or not sh[2] or st[2] != 1:
@@ -1203,7 +1204,8 @@ def window_attention(q, k, v, heads, *, kv_heads=None, left=-1, right=0, sinks=0
 
     return_lse: (out, lse), lse fp32 [B, heads, Lq] (-inf where nothing is visible), as window_attention_backward() takes it."""
     _chk_dev(q, k, v, q_len, kv_len, out)
-    _no_graph(q, k, v, out)
+    if q.requires_grad or k.requires_grad or v.requires_grad or out is not None and out.requires_grad:
+        _no_graph(q, k, v, out)
     given = out is not None
     if not given:
         out = torch.empty_like(q)
