@@ -139,7 +139,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* dy, long ldd, cons
                                                      const void* gamma, int wf32, T* dx, long lddx, float* __restrict__ parts,
                                                      long rows, int C) {
   constexpr int RPB = 256 / LPR;
-  extern __shared__ float sm[];                  // WG, LPR <= 64: 4 waves x LPR x VPL x 8 floats (at most 40 KB)
+  extern __shared__ float sm[];                  // WG, LPR <= 64: 4 waves x LPR x VPL x 8 floats (at most 24 KB)
   __shared__ float red[16];
   const int sub = threadIdx.x % LPR;
   const int nvec = (C + 7) / 8;

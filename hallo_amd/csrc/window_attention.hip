@@ -10,15 +10,18 @@
 //   O^T[d, q]   = V^T[d, :] . P^T[:, q]    A = V read transposed from LDS, B = P as the first product left it
 // The running maximum moves only when a score exceeds it by more than 6 (log2 units, so P <= 64 and the row sum stays far inside
 // fp32).  P is rounded to the storage type for the second product only, because the matrix cores take 16-bit operands at the rate that
-// this kernel lives on; the row sum adds the unrounded values, so a rounding is a relative error of half a step in one weight.  fp16's
+// this kernel lives on; the row sum adds the unrounded values, so a rounding is a relative error of half a step in one weight (on random
+// inputs the output's error against 64 bits is 1.3 to 1.4 times that of rounding the exact output once).  fp16's
 // smallest number would make it more than that: thousands of weights below 2^-25 of the largest one would be in the sum and not in the
 // product.  P therefore carries a power of two that rides in the exponent and leaves with the division by the sum (fp16, win_fwd_kernel:
 // 2^9, 64 * 2^9 is half of fp16's range; win_split_kernel, whose P is at most 1: 2^14; bf16 has fp32's range: none).
 //
 // What bounds them: win_fwd_kernel the SIMDs' issue -- MFMA and vector time (exponentials, maxima, sums, conversions) add up rather than
 // overlap, 39 + 39 % of all cycles at 128 columns, 41 + 50 % at 80, the LDS port 30 - 35 % busy.  2 x 8192 tokens, 32 / 8 heads of 128,
-// window 4096, bf16: 0.95 ms, 868 TFLOP/s; 2 x 16384 tokens, 8 heads of 80, 4097 + 1024 keys a token, fp16: 0.55 ms, 723 TFLOP/s.
-// win_split_kernel the bytes of K and V: 32 streams, 16 k window, 8 key heads of 128: 0.36 ms, 5.75 TB/s.
+// window 4096, bf16: 0.96 ms, 860 TFLOP/s; 2 x 16384 tokens, 8 heads of 80, 4097 + 1024 keys a token, fp16: 0.55 - 0.57 ms, 710 - 690 TFLOP/s
+// (the second product multiplies 96 columns for 80, 64 for 40, and 16 % of the LDS cycles are conflicts there; 128 columns: none).
+// win_split_kernel the bytes of K and V: 32 streams, 16 k window, 8 key heads of 128: 0.36 ms, 5.7 TB/s; 8 key heads of 160, 16 k keys,
+// one workgroup per CU: 0.475 ms, 5.65 TB/s.
 #include <type_traits>
 #include "window_args.h"
 #include "../../include/hallo_amd.h"
@@ -460,7 +463,7 @@ __global__ __launch_bounds__(256) void win_join_kernel(const WinArgs p) {
 
 // Which form, and how many key splits.
 // The row blocks of the split form have four waves on 32 queries, so a long range takes half as long as in blocks of 128 -- as long as all
-// of them run at once (three per CU up to 64 columns, else two; under a causal mask half of the keys on average and the longest first, so
+// of them run at once (three per CU up to 64 columns, else two -- past 128 columns only one has room, which is not counted here; under a causal mask half of the keys on average and the longest first, so
 // half as many again, twice as many where a workgroup is long).  Causal, bf16, split form / 128-query blocks: 8192 queries of one head of 64
 // (256 row blocks) 40 / 151 us, 2 x 2048 of 8 heads of 64 (1024) 30 / 43 us; of 128 columns: 1024 of 12 heads (384) 21 / 33, 2 x 1024 of
 // them (768) 31 / 36, 8192 of four heads (1024) 154 / 247, 1024 of 32 heads (1024) 38 / 34 us.  +- 100 keys, 4 x 500 of 12 heads (768):

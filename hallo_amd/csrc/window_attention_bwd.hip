@@ -9,8 +9,11 @@
 //   dq     a workgroup owns 128 queries of a head (a wave 32), the visible keys stream through LDS
 //   join   the sinks are seen by every query: their key tiles' query rows are split over workgroups, fp32 parts are added here in order
 //          (also used for all keys when there are too few key tiles to fill the chip, and for dq's keys when there are few queries)
+// P (for dV) and dS (for dQ and dK) are rounded to the storage type because the matrix cores take 16-bit operands; P, dP and dS themselves,
+// delta and all sums are fp32 (what dkv hands from role to role: see there).  On random inputs the gradients' error against 64 bits is
+// 1.4 times that of rounding the exact ones once.
 // S and dO V^T are computed in both dkv and dq (7 products where 5 would do with atomics on dQ): results do not depend on timing.
-// Bound by the SIMDs' issue as the forward pass (MFMA 40 %, vector 30 - 33 % of all cycles, LDS port 27 - 37 % busy).  2 x 8192 tokens, 32 / 8
+// Bound by the SIMDs' issue as the forward pass (MFMA 40 %, vector 30 - 34 % of all cycles, LDS port 27 - 37 % busy).  2 x 8192 tokens, 32 / 8
 // heads of 128, window 4096, bf16: 3.2 ms (dkv 1.79, dq 1.38, prep 0.06), 640 TFLOP/s of the five products that count, 900 of the seven done.
 //
 // fp16: P is 1/N over long rows and dS smaller still, below fp16's normal numbers.  Both are carried scaled by powers of two that cannot

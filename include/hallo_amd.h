@@ -445,7 +445,8 @@ int hallo_layernorm_backward(const void* dy, int64_t lddy, const void* x, int64_
  * fraction of a turn times 2^64 (axes concatenated, dims[a] / 2 each).  Pairs are (2i, 2i + 1) with interleaved = 1, else
  * (i, i + dims[a] / 2).  Columns behind the last axis are copied.  head_dim even, at most 256.
  * Positions: pos int32 [batch or 1, L, n_axes] (pos_bs = 0: one row for all entries), or pos = null and a grid whose cells are the L
- * tokens, the last axis fastest, counted from origin (the last position must fit 32 bits).  inverse = 1: negative angles, which is the gradient.  y may be x (same strides).
+ * tokens, the last axis fastest, counted from origin (the last position must fit 32 bits).  inverse = 1: negative angles, which is the
+ * gradient.  y may be x (same strides).
  * At most 2^16 heads; L below 2^31 - 64.  Rows of y must not share elements (-22), nor lie on x unless y is x.
  */
 typedef struct hallo_rope_desc {
