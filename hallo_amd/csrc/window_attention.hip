@@ -32,6 +32,13 @@ namespace {
 
 constexpr float FWD_P_EXP = 9.0f, SPLIT_P_EXP = 14.0f;       // fp16: exponent of the power of two that P carries
 
+// What the exponents of a row count from: its running maximum in log2 units, less X.  fp16: one step above, so that a rounding of a score
+// near 10^8, where a step is 8, cannot take 2^X over the type's range (1.125 * 2^-24 of a number is 0.56 to 1.13 of its step).
+template <typename T> __device__ __forceinline__ float win_base(float m, float c, float X) {
+  const float b = (m == -__builtin_inff() ? 0.0f : m * c) - X;
+  return std::is_same<T, _Float16>::value ? __builtin_fmaf(fabsf(b), 0x1.2p-24f, b) : b;
+}
+
 template <typename T, int HK>
 __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
   using V8 = typename Vec<T>::v8;
@@ -41,7 +48,8 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
   using Tile = WinTile<HK>;
   constexpr int TB = KB * Tile::PITCH, STAGE = 2 * TB;   // K | V
   constexpr int U = (KB * CH + 255) / 256;       // 16-byte pieces per thread and tensor
-  constexpr float NEG_INF = -__builtin_inff(), X = std::is_same<T, _Float16>::value ? FWD_P_EXP : 0.0f;
+  constexpr bool F16 = std::is_same<T, _Float16>::value;
+  constexpr float NEG_INF = -__builtin_inff(), X = F16 ? FWD_P_EXP : 0.0f;
   __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
   win_lds* const lds = (win_lds*)smem;
 
@@ -181,7 +189,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[db][e] *= a;
       }
-      const float mc = (m == NEG_INF ? 0.0f : m * c) - X;
+      const float mc = win_base<T>(m, c, X);
       V8 pf[NT][2];
       float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -221,7 +229,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs p) {
   // a NaN sum stays NaN
   const float inv = some ? 1.0f / l : (l != l && row < qn ? l : 0.0f);
   if (p.lse && hi == 0)
-    p.lse[((long)b * p.heads + h) * p.Lq + row] = some ? (m * c + (__builtin_amdgcn_logf(l) - X)) * 0.69314718055994530942f : (inv != 0.0f ? inv : NEG_INF);
+    p.lse[((long)b * p.heads + h) * p.Lq + row] = some ? ((F16 ? win_base<T>(m, c, X) : m * c) + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f : (inv != 0.0f ? inv : NEG_INF);
   T* O = reinterpret_cast<T*>(p.o) + (long)b * p.o_bs + (long)h * p.o_hs + (long)row * p.o_rs;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
@@ -248,8 +256,7 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   using V8 = typename Vec<T>::v8;
   constexpr int NKS = HK / 16, NDB = (HK + 31) / 32, OP = HK + 4;      // OP: pitch of the joined rows, floats
   constexpr bool F16 = std::is_same<T, _Float16>::value;
-  constexpr float NEG_INF = -__builtin_inff(), X = F16 ? SPLIT_P_EXP : 0.0f, UNDO = F16 ? 0x1p-14f : 1.0f;
-  static_assert(SPLIT_P_EXP == 14.0f, "UNDO");
+  constexpr float NEG_INF = -__builtin_inff(), X = F16 ? SPLIT_P_EXP : 0.0f;
   using Tile = WinTile<HK, HK == 112 || HK == 128 ? 16 : win_chunks(HK)>;      // eight tiles of a workgroup: two workgroups per CU at 128 columns
   constexpr int TB = 32 * Tile::PITCH, WT = 4 * 2 * TB, JT = 32 * OP * 4;      // LDS: K | V of every wave, then the joined rows
   __shared__ __attribute__((aligned(16))) unsigned char smem[WT > JT ? WT : JT];
@@ -305,8 +312,8 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
-  float m = NEG_INF, l = 0.0f;
   const float c = p.c;
+  float m = NEG_INF, mc = win_base<T>(m, c, X), l = 0.0f;
   win_lds* const kt = (win_lds*)smem + wave * 2 * TB;
   win_lds* const vt = kt + TB;
   const Tile tl(lane);
@@ -344,13 +351,13 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
       const float mn = fmaxf(m, mt);
       const float a = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
+      mc = win_base<T>(m, c, X);
       l *= a;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[db][e] *= a;
     }
-    const float mc = (m == NEG_INF ? 0.0f : m * c) - X;
     V8 pf[2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -364,12 +371,14 @@ __global__ __launch_bounds__(256, 2) void win_split_kernel(const WinArgs p) {
       for (int h2 = 0; h2 < 2; ++h2) o[db] = Vec<T>::mfma32(tl.template col<V8>(vt, h2 * 16, db), pf[h2], o[db]);
     wave_lds_order();
   }
-  l = win_half_sum(l) * UNDO;
+  // what P carried (fp16), to the bit: from here on sums and rows count from m itself
+  const float undo = F16 && m != NEG_INF ? __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -mc)) : 1.0f;
+  l = win_half_sum(l) * undo;
   if (!live) { m = NEG_INF; l = 0.0f; }          // rows without a query went along in the tiles that need no mask
   if (hi == 0) { sm_m[wave][l31] = m; sm_l[wave][l31] = l; }
   __syncthreads();                               // also: every wave is done with its V tile, the joined rows take its place
   const float M = fmaxf(fmaxf(sm_m[0][l31], sm_m[1][l31]), fmaxf(sm_m[2][l31], sm_m[3][l31]));
-  const float f = UNDO * (m == M ? 1.0f : __builtin_amdgcn_exp2f((m - M) * c));       // this wave's share (a wave without a visible key: o = 0)
+  const float f = undo * (m == M ? 1.0f : __builtin_amdgcn_exp2f((m - M) * c));       // this wave's share (a wave without a visible key: o = 0)
   float* const jt = reinterpret_cast<float*>(smem);
   for (int w4 = 0; w4 < 4; ++w4) {
     if (wave == w4) {

@@ -102,3 +102,26 @@ def test_small_far_from_large(dtype, hd, which):
         assert fits[:, cut + 1200:].all() and torch.isfinite(x[fits]).all(), name
         bad = fits & ~((x - ref).abs() <= tol)
         assert not bad.any(), (name, bad.sum().item(), bad.nonzero()[0].tolist(), ((x - ref).abs() / tol)[bad].max().item())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,Lq,H,N", [(1, 1, 2, 1000), (1, 3, 4, 6000), (9, 500, 8, 1000)])
+def test_equal_scores_of_any_size(dtype, B, Lq, H, N):
+    """All keys score the same, up to 6 10^7, where a rounding of the score in log2 units is several units: the weights are all alike and o
+    is the mean of v.  (All P of a row have one value: half a step of the storage type, the result's half a step, sums in fp32.)"""
+    from hallo_amd import ops
+    hd = 64
+    g = torch.Generator(device="cuda").manual_seed(N)
+    v = torch.randn(B, N, H, hd, generator=g, device="cuda").to(dtype)
+    mean = v.double().mean(1, keepdim=True)
+    u = torch.finfo(dtype).eps / 2
+    tol = (u * mean.abs() + (u + 4 * N * E) * v.double().abs().mean(1, keepdim=True)) * (1 + u)
+    for size in (16.0, 512.0, 768.0, 896.0):
+        q = torch.full((B, Lq, H, hd), size, device="cuda", dtype=dtype)
+        k = torch.full((B, N, H, hd), size, device="cuda", dtype=dtype)
+        for scale in (1.0, 0.9, 1.1, 1.17, -1.0):
+            k2 = -k if scale < 0 else k
+            o, lse = ops.window_attention(q, k2, v, H, right=-1, scale=abs(scale), return_lse=True)
+            s = scale * size * size * hd
+            assert ((o.double() - mean).abs() <= tol).all(), (size, scale, o[0, 0, 0, :4].tolist(), mean[0, 0, 0, :4].tolist())
+            assert ((lse.double() - (s + math.log(N))).abs() <= 16 * E * abs(s) + 1e-4).all(), (size, scale)
