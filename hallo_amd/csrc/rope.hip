@@ -348,7 +348,8 @@ extern "C" int hallo_rope(const hallo_rope_desc* d, void* stream) {
     const int64_t ext = d->L > 1 ? (d->L - 1) * d->y_rs + width : width;
     if (d->y_bs < ext) {
       if (d->L == 1 || d->y_bs < width) return -22;
-      for (int64_t b = 1; b < d->batch && b * d->y_bs / d->y_rs < d->L; ++b) {
+      const bool inside = d->y_rs >= (d->batch - 1) * d->y_bs + width;          // the batch inside of the rows
+      for (int64_t b = 1; !inside && b < d->batch && b * d->y_bs / d->y_rs < d->L; ++b) {
         const int64_t l = b * d->y_bs / d->y_rs, rest = b * d->y_bs % d->y_rs;
         if (rest < width || (l + 1 < d->L && d->y_rs - rest < width)) return -22;
       }

@@ -1049,6 +1049,8 @@ def _entries_meet(B, L, bs, rs, W):
         return False
     if L == 1 or bs < W:
         return True
+    if rs >= (B - 1) * bs + W:                   # the batch inside of the rows
+        return False
     for b in range(1, B):                        # entry b against entry 0, row 0 of either
         l, rest = divmod(b * bs, rs)
         if l >= L:

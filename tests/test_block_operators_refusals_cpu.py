@@ -224,3 +224,11 @@ def test_window_attention_splits(lib):  # noqa: F811
         assert ask(**kw) == -22, kw
     assert ask(batch=0) == 0 and ask(Lq=0) == 0 and ask() == 1
     assert ask(Lq=1, Lk=100000, left=-1) > 1 and ask(batch=64, heads=32, kv_heads=32, Lq=1000, Lk=1000) == 0
+
+
+def test_rope_batch_inside_of_the_rows_is_told_at_once():
+    """Tokens first, batch second, as a sequence-first model lays x out: no walk over the batch."""
+    import time
+    t = time.perf_counter()
+    assert not ops._entries_meet(1 << 30, 7, 64, 64 << 30, 64) and ops._entries_meet(1 << 30, 7, 64, (64 << 30) - 1, 65)
+    assert time.perf_counter() - t < 1.0
